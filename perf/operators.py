@@ -75,9 +75,10 @@ def draw(rng):
         heads = kv_heads * rng.choice((1, 2, 4, 5))
         dim = rng.choice((16, 40, 64, 80, 96, 128))
         tokens = _log_uniform(rng, 1, 4096)
-        most = 2 * 32 * 4096 * 4096 // (heads * tokens * tokens)
+        causal = rng.random() < 0.75 or heads * tokens * tokens > 32 * 4096 * 4096
+        most = (2 if causal else 1) * 32 * 4096 * 4096 // (heads * tokens * tokens)
         return dict(op=op, batch=_log_uniform(rng, 1, max(1, min(16, most))), tokens=tokens, heads=heads,
-                    kv_heads=kv_heads, dim=dim, causal=rng.random() < 0.75, ragged=rng.random() < 0.4,
+                    kv_heads=kv_heads, dim=dim, causal=causal, ragged=rng.random() < 0.4,
                     backward=rng.random() < 0.7)
     if op == "logprobs":
         vocab = _log_uniform(rng, 1000, 160000)
