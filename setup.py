@@ -18,6 +18,7 @@ setup(
             "native/*/*.cc",
             "native/*/*.hip",
             "native/*/*.h",
+            "native/hip/model/*",
             "native/collector/*.h",
             "pystacks_inject/*.py",
         ]

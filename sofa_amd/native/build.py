@@ -16,6 +16,13 @@ BIN = os.path.join(HERE, "bin")
 LIB = os.path.join(HERE, "lib")
 ROCM = os.environ.get("ROCM_PATH", "/opt/rocm")
 GFX_ARCH = "gfx950"
+# packed 32-bit arithmetic off for all device code: some of its forms have given
+# wrong results on gfx950
+HIP_FLAGS = [
+    f"--offload-arch={GFX_ARCH}",
+    "-O3",
+    "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops",
+]
 
 
 def _newer(dst: str, *srcs: str) -> bool:
@@ -140,12 +147,7 @@ def build_all(verbose: bool = False) -> None:
             continue
         if _newer(dst, *srcs):
             continue
-        cmd = [
-            hipcc,
-            f"--offload-arch={GFX_ARCH}",
-            "-O3",
-            "-std=c++17",
-        ]
+        cmd = [hipcc] + HIP_FLAGS + ["-std=c++17"]
         if dst.endswith(".so"):
             cmd += ["-fPIC", "-shared"]
         cmd += ["-o", dst] + [s for s in srcs if s.endswith(".hip")]
@@ -153,6 +155,33 @@ def build_all(verbose: bool = False) -> None:
             # --ring mode links the device-trace-ring machinery
             cmd += ["-L" + LIB, "-lsofahip", "-Wl,-rpath,$ORIGIN/../lib"]
         _run(cmd, verbose)
+
+    _build_model_kernels(hipcc, verbose)
+
+
+def _build_model_kernels(hipcc: str, verbose: bool) -> None:
+    """The operators of workloads.kernels: one object per source, compiled side
+    by side (their many variants take a minute each), then linked."""
+    src_dir = os.path.join(HERE, "hip", "model")
+    dst = os.path.join(LIB, "libsofamodel.so")
+    header = os.path.join(src_dir, "model_ops.h")
+    srcs = [os.path.join(src_dir, n) for n in sorted(os.listdir(src_dir)) if n.endswith(".hip")]
+    if _newer(dst, header, *srcs):
+        return
+    objs, running = [], []
+    for src in srcs:
+        obj = os.path.join(LIB, os.path.basename(src)[:-4] + ".o")
+        objs.append(obj)
+        if _newer(obj, header, src):
+            continue
+        cmd = [hipcc] + HIP_FLAGS + ["-std=c++20", "-fPIC", "-c", src, "-o", obj]
+        if verbose:
+            print("+ " + " ".join(cmd))
+        running.append((cmd, subprocess.Popen(cmd)))
+    failed = [cmd for cmd, p in running if p.wait() != 0]
+    if failed:
+        raise subprocess.CalledProcessError(1, failed[0])
+    _run([hipcc, f"--offload-arch={GFX_ARCH}", "-shared", "-o", dst] + objs, verbose)
 
 
 if __name__ == "__main__":

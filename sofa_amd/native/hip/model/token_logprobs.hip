@@ -1,0 +1,492 @@
+// Log probability of a given token, entropy and the most likely alternatives
+// of each row of logits, in one pass over the logits; and the gradient of the
+// first two, in one more.
+//
+// With m the running maximum of what a thread has read, it keeps
+//   s = sum e^(x - m),   a = sum e^(x - m) (x - m)
+// and moves both to a new maximum m' = m + t:  a' = e^-t (a - t s),
+// s' = e^-t s.  Joined over the row:
+//   lse = m + log s,  logprob = x_token - lse,  entropy = log s - a / s.
+// Gradient, with p = e^(x - lse), g and h the gradients of the two results:
+//   dx_j = g (1[j = token] - p_j) - h p_j (log p_j + entropy)
+//
+// What bounds it is reading the logits.  A row goes to one workgroup, or, when
+// there are few rows, to several that take a share of the vocabulary each and
+// whose results a second kernel joins.
+
+#include "model_ops.h"
+
+namespace sofa_model {
+namespace {
+
+constexpr int kThreads = 256;
+constexpr int kWaves = kThreads / kWave;
+constexpr int kMaxTop = 32;
+constexpr int kMaxParts = 64;
+
+struct LogprobArgs {
+  const void* logits;
+  const int64_t* tokens;
+  float *logprob, *entropy, *lse;
+  int64_t* top_ids;    // [rows][top], or null
+  float* top_logprobs;
+  // when parts > 1: (m, s, a) and the top candidates of each part of a row
+  float* part_sums;    // [rows][parts][3]
+  uint64_t* part_top;  // [rows][parts][top]
+  const float *dlogprob, *dentropy;  // either may be null
+  void* dlogits;                     // [rows][vocab]
+  void* stream;
+  int64_t rows, inner;        // row i is at (i / inner) outer_stride
+  int64_t outer_stride, inner_stride;  //  + (i % inner) inner_stride elements
+  int64_t grad_outer_stride, grad_inner_stride;    // of dlogprob
+  int64_t grad2_outer_stride, grad2_inner_stride;  // of dentropy
+  int64_t token_outer_stride, token_inner_stride;
+  int64_t ignore_index;
+  int vocab, top, parts, part_size;  // part_size: a multiple of kStep
+  int type, device;
+};
+
+__device__ __forceinline__ int64_t place(int64_t row, int64_t inner,
+                                         int64_t outer_stride,
+                                         int64_t inner_stride) {
+  return row / inner * outer_stride + row % inner * inner_stride;
+}
+
+struct Sums {
+  float m, s, a;
+};
+
+// A part that holds nothing but -inf has m = -inf and s = a = 0.
+__device__ __forceinline__ Sums join(Sums x, Sums y) {
+  Sums r;
+  r.m = fmaxf(x.m, y.m);
+  const float base = r.m == -INFINITY ? 0.f : r.m;
+  // max() keeps a part of -inf from 0 * -inf
+  const float tx = fmaxf(x.m - base, -1e30f), ty = fmaxf(y.m - base, -1e30f);
+  const float ex = exp2_fast(tx * kLog2e), ey = exp2_fast(ty * kLog2e);
+  r.s = x.s * ex + y.s * ey;
+  r.a = ex * (x.a + tx * x.s) + ey * (y.a + ty * y.s);
+  return r;
+}
+
+__device__ __forceinline__ Sums wave_join(Sums x) {
+#pragma unroll
+  for (int o = kWave / 2; o > 0; o >>= 1) {
+    Sums y{__shfl_xor(x.m, o), __shfl_xor(x.s, o), __shfl_xor(x.a, o)};
+    x = join(x, y);
+  }
+  return x;
+}
+
+// Takes 8 more logits; absent ones are -inf.  A NaN or +inf makes s NaN, and
+// with it every result of the row, as the definition has it.
+__device__ __forceinline__ void take(Sums& t, const float (&x)[8]) {
+  float most = x[0];
+#pragma unroll
+  for (int j = 1; j < 8; ++j) most = fmaxf(most, x[j]);
+  if (most > t.m) {
+    const float step = fmaxf(t.m - most, -1e30f);
+    const float e = exp2_fast(step * kLog2e);
+    t.a = e * (t.a + step * t.s);
+    t.s *= e;
+    t.m = most;
+  }
+  const float base = t.m == -INFINITY ? 0.f : t.m;
+#pragma unroll
+  for (int j = 0; j < 8; ++j) {
+    const float d = x[j] - base;
+    const float e = exp2_fast(d * kLog2e);
+    t.s += e;
+    t.a += e * fmaxf(d, -1e30f);
+  }
+}
+
+// ------------------------------------------------------------ alternatives
+//
+// A candidate is one 64-bit number: the logit in an order-keeping integer form
+// above, the inverted token below, so that the largest numbers are the largest
+// logits and among equals the lowest tokens.  NaN counts as the largest, -0 as
+// 0.  No candidate is 0.
+__device__ __forceinline__ uint32_t ordered(float x) {
+  const float z = x + 0.f;  // -0 becomes 0
+  uint32_t u = __float_as_uint(z);
+  if (z != z) return 0xffffffffu;
+  return u & 0x80000000u ? ~u : u | 0x80000000u;
+}
+
+__device__ __forceinline__ float unordered(uint32_t u) {
+  return u == 0xffffffffu ? __uint_as_float(0x7fc00000u)
+         : u & 0x80000000u ? __uint_as_float(u & 0x7fffffffu)
+                           : __uint_as_float(~u);
+}
+
+__device__ __forceinline__ uint64_t candidate(float x, int token) {
+  return (uint64_t) ordered(x) << 32 | (uint32_t) ~token;
+}
+
+__device__ __forceinline__ uint64_t wave_max(uint64_t x) {
+#pragma unroll
+  for (int o = kWave / 2; o > 0; o >>= 1) {
+    const uint64_t y = __shfl_xor((unsigned long long) x, o);
+    x = y > x ? y : x;
+  }
+  return x;
+}
+
+// Each wave collects candidates that beat the last of its best `top` so far,
+// and when its list is full, keeps the best `top` of it.  In random order few
+// pass after the first steps; in the worst (ascending) order every step fills
+// the list, which costs time but no result.
+constexpr int kListSize = 1024;
+constexpr int kPerLane = kListSize / kWave;
+
+struct Best {
+  uint64_t* list;  // kListSize in LDS, this wave's
+  int count;       // the same in every lane
+  uint64_t least;  // what a candidate has to beat
+  int top;
+};
+
+// Orders this wave's accesses to LDS between its lanes.
+__device__ __forceinline__ void wave_sync() {
+  __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+  __builtin_amdgcn_wave_barrier();
+  __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+}
+
+// The best `top` of the list, in falling order, to the list's front.
+__device__ __forceinline__ void keep_best(Best& b) {
+  const int lane = threadIdx.x % kWave;
+  uint64_t mine[kPerLane];
+  wave_sync();
+#pragma unroll
+  for (int k = 0; k < kPerLane; ++k) {
+    const int at = k * kWave + lane;
+    mine[k] = at < b.count ? b.list[at] : 0;
+  }
+  uint64_t last = ~0ull, next = 0;
+  for (int i = 0; i < b.top; ++i) {
+    uint64_t most = 0;
+#pragma unroll
+    for (int k = 0; k < kPerLane; ++k)
+      most = mine[k] < last && mine[k] > most ? mine[k] : most;
+    most = wave_max(most);
+    last = most;
+    if (lane == i) next = most;
+  }
+  wave_sync();
+  if (lane < b.top) b.list[lane] = next;
+  wave_sync();
+  if (b.count > b.top) b.count = b.top;
+  b.least = b.count < b.top ? 0 : last;
+}
+
+__device__ __forceinline__ void offer(Best& b, const float (&x)[8], int first,
+                                      int n) {
+  const int lane = threadIdx.x % kWave;
+  const uint64_t below = (1ull << lane) - 1;
+  uint32_t most = 0;
+  const uint32_t least = (uint32_t) (b.least >> 32);
+#pragma unroll
+  for (int j = 0; j < 8; ++j) {
+    const uint32_t u = j < n ? ordered(x[j]) : 0;
+    most = u > most ? u : most;
+  }
+  if (!__ballot(most >= least && n > 0)) return;
+#pragma unroll
+  for (int j = 0; j < 8; ++j) {
+    const uint64_t c = candidate(x[j], first + j);
+    const bool passes = j < n && c > b.least;
+    const uint64_t who = __ballot(passes);
+    if (passes) b.list[b.count + __popcll(who & below)] = c;
+    b.count += __popcll(who);
+  }
+  if (b.count > kListSize - 8 * kWave) keep_best(b);
+}
+
+template <typename T>
+__device__ __forceinline__ void finish(const LogprobArgs& a, int64_t row,
+                                       Sums t) {
+  const float log_s = log2_fast(t.s) * kLn2;
+  // a row without one allowed token: no distribution, and no NaN either
+  const bool empty = t.s == 0.f;
+  const float lse = empty ? -INFINITY : t.m + log_s;
+  const int64_t token =
+      a.tokens[place(row, a.inner, a.token_outer_stride, a.token_inner_stride)];
+  float logprob = 0.f;
+  if (token != a.ignore_index) {
+    if (token < 0 || token >= a.vocab) {
+      logprob = __uint_as_float(0x7fc00000u);  // not a token
+    } else if (empty) {
+      logprob = -INFINITY;
+    } else {
+      const T* x = static_cast<const T*>(a.logits) +
+                   place(row, a.inner, a.outer_stride, a.inner_stride);
+      logprob = ((float) x[token] - t.m) - log_s;
+    }
+  }
+  a.logprob[row] = logprob;
+  a.entropy[row] = empty ? 0.f : log_s - t.a / t.s;
+  a.lse[row] = lse;
+}
+
+__device__ __forceinline__ void put_top(const LogprobArgs& a, int64_t row,
+                                        int i, uint64_t c, Sums t) {
+  const float x = unordered((uint32_t) (c >> 32));
+  const float log_s = log2_fast(t.s) * kLn2;
+  a.top_ids[row * a.top + i] = (int64_t) (int32_t) ~(uint32_t) c;
+  a.top_logprobs[row * a.top + i] =
+      t.s == 0.f ? -INFINITY : (x - t.m) - log_s;
+}
+
+// `part` of `parts` of a row.  TOP: with alternatives.
+template <typename T, bool TOP>
+__global__ __launch_bounds__(kThreads) void logprob_kernel(LogprobArgs a) {
+  __shared__ float sums[kWaves][3];
+  __shared__ uint64_t lists[TOP ? kWaves * kListSize : 1];
+  const int lane = threadIdx.x % kWave, wave = threadIdx.x / kWave;
+  const int64_t row = blockIdx.x / a.parts;
+  const int part = blockIdx.x % a.parts;
+  const T* x = static_cast<const T*>(a.logits) +
+               place(row, a.inner, a.outer_stride, a.inner_stride);
+  const int begin = part * a.part_size;
+  const int end = min(a.vocab, begin + a.part_size);
+
+  Sums t{-INFINITY, 0.f, 0.f};
+  Best best{lists + (TOP ? wave * kListSize : 0), 0, 0, a.top};
+  constexpr int kLoads = 4;  // vectors in flight a thread
+  constexpr int kStep = kThreads * 8;
+  int at = begin;
+  for (; at + kLoads * kStep <= end; at += kLoads * kStep) {
+    float v[kLoads][8];
+#pragma unroll
+    for (int k = 0; k < kLoads; ++k)
+      load8(x + at + k * kStep + threadIdx.x * 8, v[k]);
+#pragma unroll
+    for (int k = 0; k < kLoads; ++k) {
+      take(t, v[k]);
+      if constexpr (TOP) offer(best, v[k], at + k * kStep + threadIdx.x * 8, 8);
+    }
+  }
+  for (; at < end; at += kStep) {
+    const int first = at + threadIdx.x * 8;
+    float v[8];
+    load8(x + first, v, end - first, -INFINITY);
+    take(t, v);
+    if constexpr (TOP) offer(best, v, first, end - first);
+  }
+
+  t = wave_join(t);
+  if (lane == 0) {
+    sums[wave][0] = t.m;
+    sums[wave][1] = t.s;
+    sums[wave][2] = t.a;
+  }
+  if constexpr (TOP) {
+    keep_best(best);
+    if (lane >= best.count && lane < a.top) best.list[lane] = 0;
+  }
+  __syncthreads();
+  if (wave) return;
+  t = Sums{sums[0][0], sums[0][1], sums[0][2]};
+#pragma unroll
+  for (int w = 1; w < kWaves; ++w)
+    t = join(t, Sums{sums[w][0], sums[w][1], sums[w][2]});
+  if (lane == 0) {
+    if (a.parts == 1) {
+      finish<T>(a, row, t);
+    } else {
+      float* out = a.part_sums + (row * a.parts + part) * 3;
+      out[0] = t.m;
+      out[1] = t.s;
+      out[2] = t.a;
+    }
+  }
+  if constexpr (TOP) {
+    // the waves' lists follow each other at kListSize; gather them at the front
+    const int all = kWaves * a.top;
+    uint64_t mine[kWaves * kMaxTop / kWave];
+#pragma unroll
+    for (int k = 0; k < kWaves * kMaxTop / kWave; ++k) {
+      const int i = k * kWave + lane;
+      mine[k] = i < all ? lists[i / a.top * kListSize + i % a.top] : 0;
+    }
+    wave_sync();
+#pragma unroll
+    for (int k = 0; k < kWaves * kMaxTop / kWave; ++k)
+      lists[k * kWave + lane] = mine[k];
+    wave_sync();
+    Best joined{lists, kWaves * kMaxTop, 0, a.top};
+    keep_best(joined);
+    if (lane < a.top) {
+      if (a.parts == 1)
+        put_top(a, row, lane, lists[lane], t);
+      else
+        a.part_top[(row * a.parts + part) * a.top + lane] = lists[lane];
+    }
+  }
+}
+
+// Joins the parts of a row; one wave a row.
+template <typename T, bool TOP>
+__global__ __launch_bounds__(kWave) void logprob_join_kernel(LogprobArgs a) {
+  __shared__ uint64_t list[TOP ? kListSize : 1];
+  const int lane = threadIdx.x;
+  const int64_t row = blockIdx.x;
+  Sums t{-INFINITY, 0.f, 0.f};
+  if (lane < a.parts) {
+    const float* in = a.part_sums + (row * a.parts + lane) * 3;
+    t = Sums{in[0], in[1], in[2]};
+  }
+  t = wave_join(t);
+  if (lane == 0) finish<T>(a, row, t);
+  if constexpr (TOP) {
+    Best best{list, 0, 0, a.top};
+    const uint64_t* in = a.part_top + row * a.parts * a.top;
+    const int all = a.parts * a.top;
+    for (int at = 0; at < all; at += kWave) {
+      const int i = at + lane;
+      const uint64_t c = i < all ? in[i] : 0;
+      const bool passes = c > best.least;
+      const uint64_t who = __ballot(passes);
+      if (passes) list[best.count + __popcll(who & ((1ull << lane) - 1))] = c;
+      best.count += __popcll(who);
+      if (best.count > kListSize - kWave) keep_best(best);
+    }
+    wave_sync();
+    keep_best(best);
+    if (lane < a.top) put_top(a, row, lane, list[lane], t);
+  }
+}
+
+template <typename T>
+__global__ __launch_bounds__(kThreads) void logprob_backward_kernel(
+    LogprobArgs a) {
+  const int64_t row = blockIdx.x / a.parts;
+  const int part = blockIdx.x % a.parts;
+  const T* x = static_cast<const T*>(a.logits) +
+               place(row, a.inner, a.outer_stride, a.inner_stride);
+  T* dx = static_cast<T*>(a.dlogits) + row * a.vocab;
+  const int begin = part * a.part_size;
+  const int end = min(a.vocab, begin + a.part_size);
+  const float lse = a.lse[row], entropy = a.entropy[row];
+  int64_t token =
+      a.tokens[place(row, a.inner, a.token_outer_stride, a.token_inner_stride)];
+  float g = 0.f, h = 0.f;
+  if (a.dlogprob && token != a.ignore_index)
+    g = a.dlogprob[place(row, a.inner, a.grad_outer_stride,
+                         a.grad_inner_stride)];
+  if (a.dentropy)
+    h = a.dentropy[place(row, a.inner, a.grad2_outer_stride,
+                         a.grad2_inner_stride)];
+  // nothing to pass on, or an empty row: zeros, and nothing is read
+  const bool zero = (g == 0.f && h == 0.f) || lse == -INFINITY;
+  // dx = g 1[token] - p (g + h entropy + h log p)
+  const float base = g + h * entropy;
+
+  constexpr int kLoads = 4;
+  constexpr int kStep = kThreads * 8;
+  auto gradient = [&](float (&v)[8], int first) {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      const float logp = v[j] - lse;
+      const float p = exp2_fast(logp * kLog2e);
+      // a masked logit has p = 0 and log p = -inf
+      float d = -p * (base + h * fmaxf(logp, -1e30f));
+      if (first + j == token) d += g;
+      v[j] = zero ? 0.f : d;
+    }
+  };
+  int at = begin;
+  for (; at + kLoads * kStep <= end; at += kLoads * kStep) {
+    float v[kLoads][8];
+#pragma unroll
+    for (int k = 0; k < kLoads; ++k) {
+      if (!zero) load8(x + at + k * kStep + threadIdx.x * 8, v[k]);
+    }
+#pragma unroll
+    for (int k = 0; k < kLoads; ++k) {
+      const int first = at + k * kStep + threadIdx.x * 8;
+      gradient(v[k], first);
+      store8(dx + first, v[k]);
+    }
+  }
+  for (; at < end; at += kStep) {
+    const int first = at + threadIdx.x * 8;
+    float v[8];
+    load8(x + first, v, zero ? 0 : end - first);
+    gradient(v, first);
+    store8(dx + first, v, end - first);
+  }
+}
+
+template <typename T>
+int forward(const LogprobArgs& a) {
+  const hipStream_t stream = static_cast<hipStream_t>(a.stream);
+  const dim3 grid((unsigned) (a.rows * a.parts));
+  if (a.top)
+    hipLaunchKernelGGL((logprob_kernel<T, true>), grid, dim3(kThreads), 0,
+                       stream, a);
+  else
+    hipLaunchKernelGGL((logprob_kernel<T, false>), grid, dim3(kThreads), 0,
+                       stream, a);
+  int status = (int) hipGetLastError();
+  if (status || a.parts == 1) return status;
+  if (a.top)
+    hipLaunchKernelGGL((logprob_join_kernel<T, true>), dim3((unsigned) a.rows),
+                       dim3(kWave), 0, stream, a);
+  else
+    hipLaunchKernelGGL((logprob_join_kernel<T, false>), dim3((unsigned) a.rows),
+                       dim3(kWave), 0, stream, a);
+  return (int) hipGetLastError();
+}
+
+template <typename T>
+int backward(const LogprobArgs& a) {
+  hipLaunchKernelGGL(logprob_backward_kernel<T>,
+                     dim3((unsigned) (a.rows * a.parts)), dim3(kThreads), 0,
+                     static_cast<hipStream_t>(a.stream), a);
+  return (int) hipGetLastError();
+}
+
+bool sound(const LogprobArgs* a) {
+  return a && a->logits && a->tokens && a->logprob && a->entropy && a->lse &&
+         a->rows > 0 && a->inner > 0 && a->vocab > 0 && a->vocab <= 1 << 30 &&
+         a->parts > 0 &&
+         a->parts <= kMaxParts && a->part_size > 0 &&
+         (int64_t) a->parts * a->part_size >= a->vocab &&
+         (int64_t) (a->parts - 1) * a->part_size < a->vocab &&
+         a->rows <= INT32_MAX / a->parts;
+}
+
+}  // namespace
+}  // namespace sofa_model
+
+extern "C" {
+
+int sofa_logprob_forward(const sofa_model::LogprobArgs* a) {
+  using namespace sofa_model;
+  if (!sound(a) || a->top < 0 || a->top > kMaxTop || a->top > a->vocab ||
+      (a->top && !(a->top_ids && a->top_logprobs)) ||
+      (a->parts > 1 && !(a->part_sums && (a->part_top || !a->top))))
+    return kBadArgument;
+  DeviceGuard guard(a->device);
+  if (guard.status()) return guard.status();
+  if (a->type == kFloat32) return forward<float>(*a);
+  if (a->type == kBFloat16) return forward<bf16>(*a);
+  if (a->type == kFloat16) return forward<fp16>(*a);
+  return kBadArgument;
+}
+
+int sofa_logprob_backward(const sofa_model::LogprobArgs* a) {
+  using namespace sofa_model;
+  if (!sound(a) || !a->dlogits) return kBadArgument;
+  DeviceGuard guard(a->device);
+  if (guard.status()) return guard.status();
+  if (a->type == kFloat32) return backward<float>(*a);
+  if (a->type == kBFloat16) return backward<bf16>(*a);
+  if (a->type == kFloat16) return backward<fp16>(*a);
+  return kBadArgument;
+}
+
+}  // extern "C"

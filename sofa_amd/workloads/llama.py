@@ -9,6 +9,11 @@ so no sharding complexity is needed on this hardware).
 
 Run directly for a profiled step stress:
     sofa stat "python -m sofa_amd.workloads.llama --layers 8 --steps 3"
+
+`--kernels hip` (`Llama(kernels="hip")`) runs attention, the residual norms and
+the loss as the fused kernels of workloads.kernels in place of ATen: the same
+parameters and mathematics in about a tenth of the kernel launches outside the
+matrix products, for profiling a step as a tuned trainer would run it.
 """
 
 from __future__ import annotations
@@ -52,9 +57,16 @@ def apply_rope(x, cos, sin):
     return out
 
 
+def hip_kernels():
+    from sofa_amd.workloads import kernels
+
+    return kernels
+
+
 class Attention(nn.Module):
-    def __init__(self, dim: int, n_heads: int, n_kv_heads: int):
+    def __init__(self, dim: int, n_heads: int, n_kv_heads: int, kernels: str = "torch"):
         super().__init__()
+        self.kernels = kernels
         self.n_heads = n_heads
         self.n_kv = n_kv_heads
         self.hd = dim // n_heads
@@ -70,6 +82,10 @@ class Attention(nn.Module):
         v = self.wv(x).view(B, T, self.n_kv, self.hd).transpose(1, 2)
         q = apply_rope(q, cos, sin)
         k = apply_rope(k, cos, sin)
+        if self.kernels == "hip":
+            # the result is token-major: the reshape below is a view
+            o = hip_kernels().attention(q, k, v)
+            return self.wo(o.transpose(1, 2).reshape(B, T, C))
         # GQA: SDPA broadcasts kv heads with enable_gqa-free repeat
         k = k.repeat_interleave(self.n_heads // self.n_kv, dim=1)
         v = v.repeat_interleave(self.n_heads // self.n_kv, dim=1)
@@ -89,10 +105,10 @@ class MLP(nn.Module):
 
 
 class Block(nn.Module):
-    def __init__(self, dim, n_heads, n_kv, hidden):
+    def __init__(self, dim, n_heads, n_kv, hidden, kernels: str = "torch"):
         super().__init__()
         self.attn_norm = RMSNorm(dim)
-        self.attn = Attention(dim, n_heads, n_kv)
+        self.attn = Attention(dim, n_heads, n_kv, kernels)
         self.mlp_norm = RMSNorm(dim)
         self.mlp = MLP(dim, hidden)
 
@@ -111,11 +127,15 @@ class Llama(nn.Module):
         n_kv_heads: int = 8,
         hidden: int = 14336,
         max_seq: int = 8192,
+        kernels: str = "torch",
     ):
         super().__init__()
+        if kernels not in ("torch", "hip"):
+            raise ValueError(f"kernels has to be 'torch' or 'hip', got {kernels!r}")
+        self.kernels = kernels
         self.embed = nn.Embedding(vocab, dim)
         self.blocks = nn.ModuleList(
-            [Block(dim, n_heads, n_kv_heads, hidden) for _ in range(n_layers)]
+            [Block(dim, n_heads, n_kv_heads, hidden, kernels) for _ in range(n_layers)]
         )
         self.norm = RMSNorm(dim)
         self.lm_head = nn.Linear(dim, vocab, bias=False)
@@ -125,13 +145,38 @@ class Llama(nn.Module):
 
     def forward(self, tokens):
         x = self.embed(tokens)
+        if self.kernels == "hip":
+            return self.lm_head(self._hip_blocks(x))
         for b in self.blocks:
             x = b(x, self.rope_cos, self.rope_sin)
         return self.lm_head(self.norm(x))
 
+    def _hip_blocks(self, x):
+        """The blocks and the last norm, with each sum onto the residual stream
+        fused into the norm that follows it.  Norms leave in the type that the
+        products take, which autocast would cast them to."""
+        dt = torch.get_autocast_dtype("cuda") if torch.is_autocast_enabled("cuda") else x.dtype
+        add_norm = hip_kernels().residual_norm
+        norms = [n for b in self.blocks for n in (b.attn_norm, b.mlp_norm)] + [self.norm]
+        branch = None
+        for i, norm in enumerate(norms):
+            x, h = add_norm(x, branch, norm.weight, eps=norm.eps, out_dtype=dt)
+            if norm is not self.norm:
+                b = self.blocks[i // 2]
+                branch = b.mlp(h) if i % 2 else b.attn(h, self.rope_cos, self.rope_sin)
+        return h
 
-def build_llama8b(device="cuda", n_layers: int = 32) -> Llama:
-    m = Llama(n_layers=n_layers)
+    def loss(self, tokens, target):
+        """Mean cross entropy of the targets."""
+        logits = self(tokens)
+        if self.kernels == "hip":
+            logprob = hip_kernels().token_logprobs(logits, target).logprob
+            return -logprob.sum() / (target != -100).sum()
+        return F.cross_entropy(logits.view(-1, logits.shape[-1]).float(), target.view(-1))
+
+
+def build_llama8b(device="cuda", n_layers: int = 32, kernels: str = "torch") -> Llama:
+    m = Llama(n_layers=n_layers, kernels=kernels)
     return m.to(device)
 
 
@@ -142,18 +187,19 @@ def main() -> int:
     ap.add_argument("--batch", type=int, default=2)
     ap.add_argument("--seq", type=int, default=4096)
     ap.add_argument("--device", default="cuda")
+    ap.add_argument("--kernels", choices=["torch", "hip"], default="torch",
+                    help="hip: attention, norms and loss as fused HIP kernels (needs the GPU)")
     args = ap.parse_args()
 
     torch.manual_seed(0)
     device = args.device if torch.cuda.is_available() or args.device == "cpu" else "cpu"
-    model = build_llama8b(device=device, n_layers=args.layers)
+    model = build_llama8b(device=device, n_layers=args.layers, kernels=args.kernels)
     opt = torch.optim.AdamW(model.parameters(), lr=1e-4)
     tokens = torch.randint(0, 128256, (args.batch, args.seq), device=device)
     target = torch.randint(0, 128256, (args.batch, args.seq), device=device)
     for i in range(args.steps):
         with torch.autocast(device_type="cuda" if device != "cpu" else "cpu", dtype=torch.bfloat16):
-            logits = model(tokens)
-            loss = F.cross_entropy(logits.view(-1, logits.shape[-1]).float(), target.view(-1))
+            loss = model.loss(tokens, target)
         opt.zero_grad(set_to_none=True)
         loss.backward()
         opt.step()

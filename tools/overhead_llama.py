@@ -25,6 +25,7 @@ def main() -> int:
     ap.add_argument("--batch", type=int, default=2)
     ap.add_argument("--seq", type=int, default=2048)
     ap.add_argument("--tracer", choices=["sdk", "lite"], default="lite")
+    ap.add_argument("--kernels", choices=["torch", "hip"], default="torch")
     args = ap.parse_args()
 
     logdir = os.path.join(REPO, "gpurun_out", "llama_ovh")
@@ -34,21 +35,19 @@ def main() -> int:
     setup_tracer_env(logdir, args.tracer)
 
     import torch
-    import torch.nn.functional as F
 
     from sofa_amd.workloads.llama import build_llama8b
 
     lib = TracerCtl(args.tracer)
 
-    model = build_llama8b(device="cuda", n_layers=args.layers)
+    model = build_llama8b(device="cuda", n_layers=args.layers, kernels=args.kernels)
     opt = torch.optim.AdamW(model.parameters(), lr=1e-4)
     tokens = torch.randint(0, 128256, (args.batch, args.seq), device="cuda")
     target = torch.randint(0, 128256, (args.batch, args.seq), device="cuda")
 
     def step():
         with torch.autocast(device_type="cuda", dtype=torch.bfloat16):
-            logits = model(tokens)
-            loss = F.cross_entropy(logits.view(-1, logits.shape[-1]).float(), target.view(-1))
+            loss = model.loss(tokens, target)
         opt.zero_grad(set_to_none=True)
         loss.backward()
         opt.step()
