@@ -21,7 +21,12 @@
 // of each 16.  Its A operand is read from LDS with ds_read_b64_tr_b16, which
 // gives a lane 4 rows of one column, in that same order.  P and dS are rounded
 // to bf16 for it: 2^-8 relative at most, as in the results themselves; sums
-// stay in 32 bits.
+// stay in 32 bits.  Only delta, which dP - delta almost cancels in short rows,
+// takes more of o than its 8 bits: the forward pass keeps what the rounding
+// took off as well (with o's own rounding dQ and dK of 32 tokens were 3.1e-3
+// off, 1.9 times what the rounding of the results is).
+// delta, though, is a difference that short rows almost cancel: it is taken
+// of o in 16 bits, kept as o and what its rounding took off.
 
 #include "model_ops.h"
 
@@ -31,6 +36,7 @@ namespace {
 struct AttentionArgs {
   const bf16 *q, *k, *v;  // [batch][heads][tokens][dim] by strides, dim dense
   bf16* o;
+  bf16* o_low;            // what rounding took off o, laid out like it; or null
   float* lse;             // [batch][heads][tokens], base 2; +inf: no keys
   const int* lengths;     // [batch] valid tokens, or null
   const bf16* dout;
@@ -42,6 +48,7 @@ struct AttentionArgs {
   float scale;
   int batch, heads, kv_heads, tokens, dim, causal, device;
 };
+static_assert(sizeof(AttentionArgs) == 328, "as the caller packs it");
 
 typedef bf16 bf16x4 __attribute__((ext_vector_type(4)));
 typedef bf16 bf16x8 __attribute__((ext_vector_type(8)));
@@ -155,21 +162,30 @@ __device__ __forceinline__ void load_row(bf16x8 (&x)[DP / 16], const bf16* row,
 }
 
 // The transposed result of a wave: the lane's row, in DP / 32 blocks of D;
-// zeros in a row that is not valid, whatever was computed for it
+// zeros in a row that is not valid, whatever was computed for it.  `low`, if
+// there is one, takes what the rounding took off.
 template <int DP>
 __device__ __forceinline__ void store_row(bf16* row,
                                           const floatx16 (&acc)[DP / 32],
-                                          float factor, bool valid, int dim) {
+                                          float factor, bool valid, int dim,
+                                          bf16* low = nullptr) {
   const int h = threadIdx.x % kWave / 32;
 #pragma unroll
   for (int b = 0; b < DP / 32; ++b)
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       const int at = b * 32 + i * 8 + h * 4;
-      bf16x4 x;
+      bf16x4 x, rest;
 #pragma unroll
-      for (int j = 0; j < 4; ++j) x[j] = (bf16) (valid ? acc[b][i * 4 + j] * factor : 0.f);
-      if (at < dim) *reinterpret_cast<bf16x4*>(row + at) = x;
+      for (int j = 0; j < 4; ++j) {
+        const float y = valid ? acc[b][i * 4 + j] * factor : 0.f;
+        x[j] = (bf16) y;
+        rest[j] = (bf16) (y - (float) x[j]);
+      }
+      if (at < dim) {
+        *reinterpret_cast<bf16x4*>(row + at) = x;
+        if (low) *reinterpret_cast<bf16x4*>(low + at) = rest;
+      }
     }
 }
 
@@ -276,9 +292,10 @@ __global__ __launch_bounds__(kThreads, 2) void attention_forward_kernel(
   if (row >= a.tokens) return;
   l += other_half(l);
   const bool valid = row < n;
-  store_row<DP>(a.o + batch * a.o_stride[0] + head * a.o_stride[1] +
-                    (int64_t) row * a.o_stride[2],
-                acc, 1.f / l, valid, a.dim);
+  const int64_t o_at = batch * a.o_stride[0] + head * a.o_stride[1] +
+                       (int64_t) row * a.o_stride[2];
+  store_row<DP>(a.o + o_at, acc, 1.f / l, valid, a.dim,
+                a.o_low ? a.o_low + o_at : nullptr);
   if (a.lse && h == 0)
     a.lse[(int64_t) bh * a.tokens + row] =
         valid ? m + log2_fast(l) : INFINITY;
@@ -307,7 +324,7 @@ __global__ __launch_bounds__(kThreads, 2) void attention_dq_kernel(
   bf16x8 q[DP / 16], dout[DP / 16];
   float delta = 0.f;
   {
-    bf16x8 o[DP / 16];
+    bf16x8 o[DP / 16], o_low[DP / 16];
     load_row<DP>(q,
                  a.q + batch * a.q_stride[0] + head * a.q_stride[1] +
                      (int64_t) row * a.q_stride[2],
@@ -316,14 +333,15 @@ __global__ __launch_bounds__(kThreads, 2) void attention_dq_kernel(
                  a.dout + batch * a.dout_stride[0] + head * a.dout_stride[1] +
                      (int64_t) row * a.dout_stride[2],
                  valid, a.dim);
-    load_row<DP>(o,
-                 a.o + batch * a.o_stride[0] + head * a.o_stride[1] +
-                     (int64_t) row * a.o_stride[2],
-                 valid, a.dim);
+    const int64_t o_at = batch * a.o_stride[0] + head * a.o_stride[1] +
+                         (int64_t) row * a.o_stride[2];
+    load_row<DP>(o, a.o + o_at, valid, a.dim);
+    load_row<DP>(o_low, a.o_low + o_at, valid, a.dim);
 #pragma unroll
     for (int s = 0; s < DP / 16; ++s)
 #pragma unroll
-      for (int j = 0; j < 8; ++j) delta += (float) dout[s][j] * (float) o[s][j];
+      for (int j = 0; j < 8; ++j)
+        delta += (float) dout[s][j] * ((float) o[s][j] + (float) o_low[s][j]);
     delta += other_half(delta);
   }
   const int64_t at = (int64_t) bh * a.tokens + row;
@@ -534,7 +552,7 @@ int sofa_attention_forward(const sofa_model::AttentionArgs* a) {
 
 int sofa_attention_backward(const sofa_model::AttentionArgs* a) {
   using namespace sofa_model;
-  if (!sound(a) || !a->dout || !a->lse || !a->delta || !a->dq || !a->dk ||
+  if (!sound(a) || !a->dout || !a->o_low || !a->lse || !a->delta || !a->dq || !a->dk ||
       !a->dv)
     return kBadArgument;
   DeviceGuard guard(a->device);

@@ -35,8 +35,9 @@ struct NormArgs {
   int teams_per_group;       // backward: teams that share a gate's rows
   int device;
 };
+static_assert(sizeof(NormArgs) == 192, "as the caller packs it");
 
-// Sums of N <= 3 values over a team, in every thread of it.  `parity` alternates
+// Sums of N <= 2 values over a team, in every thread of it.  `parity` alternates
 // between calls, so that one barrier is enough: a buffer is written again
 // only after the barrier of the call between.
 template <int TEAM, int N>
@@ -46,19 +47,19 @@ __device__ __forceinline__ void team_sum(float (&v)[N], float* smem,
   for (int k = 0; k < N; ++k) v[k] = wave_sum(v[k]);
   if constexpr (TEAM > kWave) {
     constexpr int kWaves = TEAM / kWave;
-    float* buf = smem + parity * kWaves * 3;
+    float* buf = smem + parity * kWaves * 2;
     parity ^= 1;
     const int wave = threadIdx.x / kWave;
     if (threadIdx.x % kWave == 0) {
 #pragma unroll
-      for (int k = 0; k < N; ++k) buf[wave * 3 + k] = v[k];
+      for (int k = 0; k < N; ++k) buf[wave * 2 + k] = v[k];
     }
     __syncthreads();
 #pragma unroll
     for (int k = 0; k < N; ++k) {
       float s = 0.f;
 #pragma unroll
-      for (int w = 0; w < kWaves; ++w) s += buf[w * 3 + k];
+      for (int w = 0; w < kWaves; ++w) s += buf[w * 2 + k];
       v[k] = s;
     }
   }
@@ -71,7 +72,7 @@ template <typename X, typename B, typename Y, int TEAM, int VPT>
 __global__ __launch_bounds__(kBlock<TEAM>) void norm_forward_kernel(
     NormArgs a) {
   constexpr int kTeams = kBlock<TEAM> / TEAM;
-  __shared__ float smem[TEAM > kWave ? 2 * 3 * TEAM / kWave : 1];
+  __shared__ float smem[TEAM > kWave ? 2 * 2 * TEAM / kWave : 1];
   const int lane = threadIdx.x % TEAM;
   const int64_t team = (int64_t) blockIdx.x * kTeams + threadIdx.x / TEAM;
   const int64_t teams = (int64_t) gridDim.x * kTeams;
@@ -152,12 +153,14 @@ __global__ __launch_bounds__(kBlock<TEAM>) void norm_forward_kernel(
 // A team takes consecutive rows of one gate's group, so that the gate and its
 // gradient stay in registers too.
 // EXTRA: the branch has a norm or a gate; without them their registers
-// (5 of 8 vectors) are not held.
+// (5 of 8 vectors) are not held.  x is r where that is held in 32 bits (or there
+// is no branch); a 16-bit r has lost what the gradients of the weights need,
+// so x is x then and r is summed up again.
 template <typename X, typename B, typename Y, int TEAM, int VPT, bool EXTRA>
 __global__ __launch_bounds__(kBlock<TEAM>) void norm_backward_kernel(
     NormArgs a) {
   constexpr int kTeams = kBlock<TEAM> / TEAM;
-  __shared__ float smem[TEAM > kWave ? 2 * 3 * TEAM / kWave : 1];
+  __shared__ float smem[TEAM > kWave ? 2 * 2 * TEAM / kWave : 1];
   const int lane = threadIdx.x % TEAM;
   const int64_t teams = a.rows / a.group_rows * a.teams_per_group;
   const int64_t team = (int64_t) blockIdx.x * kTeams + threadIdx.x / TEAM;
@@ -192,7 +195,7 @@ __global__ __launch_bounds__(kBlock<TEAM>) void norm_backward_kernel(
   }
 
   for (int64_t row = first; row < last; ++row) {
-    const X* r = static_cast<const X*>(a.x) + row * a.dim;
+    const X* x = static_cast<const X*>(a.x) + row * a.dim;
     const Y* dy = static_cast<const Y*>(a.dy) + row * a.dim;
     const X* dr = static_cast<const X*>(a.dr) + row * a.dim;
     const B* branch = static_cast<const B*>(a.branch) + row * a.dim;
@@ -202,19 +205,49 @@ __global__ __launch_bounds__(kBlock<TEAM>) void norm_backward_kernel(
 #pragma unroll
     for (int v = 0; v < VPT; ++v) {
       const int at = (v * TEAM + lane) * 8;
-      load8(r + at, z[v], a.dy ? a.dim - at : 0);
+      load8(x + at, z[v], a.dim - at);
       load8(dy + at, d[v], a.dy ? a.dim - at : 0);
       load8(dr + at, in[v], a.dr ? a.dim - at : 0);
       if constexpr (EXTRA) load8(branch + at, h[v], a.dim - at);
     }
-    float sum[3] = {0.f, 0.f, 0.f};
+    // without a norm of the branch: its unit is h, and no mean to take off
+    float sh = 1.f, ch = 0.f;
+    if constexpr (EXTRA) {
+      if (a.post) {
+        float sums[1] = {0.f};
+#pragma unroll
+        for (int v = 0; v < VPT; ++v)
+#pragma unroll
+          for (int j = 0; j < 8; ++j) sums[0] += h[v][j] * h[v][j];
+        team_sum<TEAM>(sums, smem, parity);
+        sh = rsqrtf(sums[0] * inv_dim + a.eps);
+      }
+    }
+    if constexpr (sizeof(X) == 2) {
+      if (a.branch) {
+#pragma unroll
+        for (int v = 0; v < VPT; ++v) {
+          const int at = (v * TEAM + lane) * 8;
+          if constexpr (EXTRA) {
+#pragma unroll
+            for (int j = 0; j < 8; ++j)
+              z[v][j] += gate[v][j] * (sh * post[v][j]) * h[v][j];
+          } else {
+            float hs[8];
+            load8(branch + at, hs, a.dim - at);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) z[v][j] += a.scale * hs[j];
+          }
+        }
+      }
+    }
+    float sum[2] = {0.f, 0.f};
 #pragma unroll
     for (int v = 0; v < VPT; ++v)
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
         sum[0] += z[v][j] * z[v][j];
         sum[1] += d[v][j] * weight[v][j] * z[v][j];
-        if constexpr (EXTRA) sum[2] += h[v][j] * h[v][j];
       }
     team_sum<TEAM>(sum, smem, parity);
     const float s = rsqrtf(sum[0] * inv_dim + a.eps);
@@ -239,8 +272,6 @@ __global__ __launch_bounds__(kBlock<TEAM>) void norm_backward_kernel(
         store8(dbranch + at, d[v], a.dim - at);
       }
     } else {
-      // without a norm of the branch: unit = h, and no mean to take off
-      float sh = 1.f, ch = 0.f;
       if (a.post) {
         float sums[1] = {0.f};
 #pragma unroll
@@ -249,7 +280,6 @@ __global__ __launch_bounds__(kBlock<TEAM>) void norm_backward_kernel(
           for (int j = 0; j < 8; ++j)
             sums[0] += d[v][j] * gate[v][j] * post[v][j] * h[v][j];
         team_sum<TEAM>(sums, smem, parity);
-        sh = rsqrtf(sum[2] * inv_dim + a.eps);
         ch = sh * sh * sh * inv_dim * sums[0];
       }
 #pragma unroll
@@ -424,19 +454,6 @@ int sofa_norm_forward(const sofa_model::NormArgs* a) {
   DeviceGuard guard(a->device);
   if (guard.status()) return guard.status();
   return by_types(*a, Forward{*a});
-}
-
-// Teams that the backward pass gives each gate's rows; the caller sizes
-// `partial` by it: sums * (rows / group_rows) * teams * dim floats.
-// About 512 workgroups fill the card twice; more would only add partial rows.
-int sofa_norm_backward_teams(int64_t rows, int64_t group_rows, int dim) {
-  if (rows <= 0 || group_rows <= 0 || rows % group_rows) return 0;
-  const int64_t groups = rows / group_rows;
-  const int64_t most = dim <= 1024 ? 2048 : 512;
-  int64_t teams = most / groups;
-  if (teams < 1) teams = 1;
-  if (teams > group_rows) teams = group_rows;
-  return (int) teams;
 }
 
 int sofa_norm_backward(const sofa_model::NormArgs* a) {

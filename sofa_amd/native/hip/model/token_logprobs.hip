@@ -45,6 +45,7 @@ struct LogprobArgs {
   int vocab, top, parts, part_size;  // part_size: a multiple of kStep
   int type, device;
 };
+static_assert(sizeof(LogprobArgs) == 216, "as the caller packs it");
 
 __device__ __forceinline__ int64_t place(int64_t row, int64_t inner,
                                          int64_t outer_stride,

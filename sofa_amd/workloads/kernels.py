@@ -19,6 +19,7 @@ from __future__ import annotations
 import ctypes
 import math
 import os
+import struct
 from typing import NamedTuple, Optional, Tuple
 
 import torch
@@ -31,39 +32,12 @@ MAX_TOP = 32
 MAX_NORM_DIM = 16384
 MAX_VOCAB = 1 << 30
 
-_P, _I, _L, _F = ctypes.c_void_p, ctypes.c_int, ctypes.c_int64, ctypes.c_float
-
-
-def _struct(name, *fields):
-    """A ctypes structure out of (type, "names ...") pairs, in order."""
-    return type(name, (ctypes.Structure,), {
-        "_fields_": [(n, t) for t, names in fields for n in names.split()]
-    })
-
-
-# the argument structures of the C entries, field by field
-_AttentionArgs = _struct(
-    "_AttentionArgs",
-    (_P, "q k v o lse lengths dout delta dq dk dv stream"),
-    (_L * 3, "q_stride k_stride v_stride o_stride dout_stride dq_stride dk_stride dv_stride"),
-    (_F, "scale"),
-    (_I, "batch heads kv_heads tokens dim causal device"),
-)
-_LogprobArgs = _struct(
-    "_LogprobArgs",
-    (_P, "logits tokens logprob entropy lse top_ids top_logprobs part_sums part_top "
-         "dlogprob dentropy dlogits stream"),
-    (_L, "rows inner outer_stride inner_stride grad_outer_stride grad_inner_stride "
-         "grad2_outer_stride grad2_inner_stride token_outer_stride token_inner_stride ignore_index"),
-    (_I, "vocab top parts part_size type device"),
-)
-_NormArgs = _struct(
-    "_NormArgs",
-    (_P, "x branch weight post gate r y dr dy dx dbranch partial dweight dpost dgate stream"),
-    (_L, "rows group_rows"),
-    (_F, "eps scale"),
-    (_I, "dim x_type branch_type y_type weight_type post_type gate_type teams_per_group device"),
-)
+# The argument structures of the C entries, packed in one call each: pointers,
+# then 64-bit, 32-bit floating and 32-bit whole numbers, in the order of their
+# declarations in native/hip/model.  "0q" pads the end as C does.
+_ATTENTION = struct.Struct("13P24qf7i0q")
+_LOGPROBS = struct.Struct("13P11q6i0q")
+_NORM = struct.Struct("16P2q2f9i0q")
 
 _lib_handle = None
 
@@ -81,22 +55,30 @@ def _lib():
         for name in ("attention_forward", "attention_backward", "logprob_forward",
                      "logprob_backward", "norm_forward", "norm_backward"):
             entry = getattr(lib, "sofa_" + name)
-            entry.argtypes, entry.restype = [_P], _I
-        lib.sofa_norm_backward_teams.argtypes = [_L, _L, _I]
-        lib.sofa_norm_backward_teams.restype = _I
+            entry.argtypes, entry.restype = [ctypes.c_char_p], ctypes.c_int
         _lib_handle = lib
     return _lib_handle
 
 
-def _call(name: str, args) -> None:
-    status = getattr(_lib(), name)(ctypes.addressof(args))
+def _call(name: str, args: bytes) -> None:
+    status = getattr(_lib_handle or _lib(), name)(args)
     if status:
         what = "bad argument" if status < 0 else f"HIP error {status}"
         raise RuntimeError(f"{name} failed: {what}")
 
 
-def _stream(device: torch.device) -> int:
-    return torch.cuda.current_stream(device).cuda_stream
+# a torch.cuda.Stream object for each call would cost as much as the launch
+_stream = torch._C._cuda_getCurrentRawStream
+
+
+def _once(backward):
+    """A backward pass that is itself recorded only to refuse a second one."""
+    recorded = torch.autograd.function.once_differentiable(backward)
+
+    def either(ctx, *grads):
+        return (recorded if torch.is_grad_enabled() else backward)(ctx, *grads)
+
+    return either
 
 
 def _on_gpu(what: str, first: torch.Tensor, **others: Optional[torch.Tensor]) -> None:
@@ -107,8 +89,8 @@ def _on_gpu(what: str, first: torch.Tensor, **others: Optional[torch.Tensor]) ->
             raise ValueError(f"{what}: {name} is on {t.device}, not on {first.device}")
 
 
-def _ptr(t: Optional[torch.Tensor]) -> Optional[int]:
-    return None if t is None else t.data_ptr()
+def _ptr(t: Optional[torch.Tensor]) -> int:
+    return 0 if t is None else t.data_ptr()
 
 
 def _recorded(*tensors: Optional[torch.Tensor]) -> bool:
@@ -119,62 +101,62 @@ def _recorded(*tensors: Optional[torch.Tensor]) -> bool:
 # ------------------------------------------------------------------ attention
 def _rows16(t: torch.Tensor) -> torch.Tensor:
     """t, or a copy, with dense rows that start at multiples of 16 bytes."""
-    if (t.stride(3) == 1 and t.data_ptr() % 16 == 0
-            and all(s % 8 == 0 or n == 1 for s, n in zip(t.stride()[:3], t.shape[:3]))):
+    a, b, c, dense = t.stride()
+    # the stride of an axis of one is never used
+    if dense == 1 and t.data_ptr() % 16 == 0 and (
+            (a | b | c) % 8 == 0 or all(s % 8 == 0 or n == 1 for s, n in zip((a, b, c), t.shape))):
         return t
-    return t.contiguous()
+    return t.clone(memory_format=torch.contiguous_format)
 
 
-def _token_major(batch: int, heads: int, tokens: int, dim: int, like: torch.Tensor) -> torch.Tensor:
+def _token_major(like: torch.Tensor) -> torch.Tensor:
     """(batch, heads, tokens, dim) laid out as (batch, tokens, heads, dim): what
     the projection behind it reads as one matrix without a copy."""
-    return torch.empty((batch, tokens, heads, dim), dtype=like.dtype, device=like.device).transpose(1, 2)
+    batch, heads, tokens, dim = like.shape
+    return like.new_empty_strided(like.shape, (tokens * heads * dim, dim, heads * dim, 1))
 
 
-def _attention_args(q, k, v, o, lse, lengths, scale, causal):
-    a = _AttentionArgs()
-    a.q, a.k, a.v, a.o = q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr()
-    a.lse, a.lengths = _ptr(lse), _ptr(lengths)
-    a.q_stride[:], a.k_stride[:] = q.stride()[:3], k.stride()[:3]
-    a.v_stride[:], a.o_stride[:] = v.stride()[:3], o.stride()[:3]
-    a.scale, a.causal = scale, causal
-    a.batch, a.heads, a.tokens, a.dim = q.shape
-    a.kv_heads = k.shape[1]
-    a.device = q.device.index
-    a.stream = _stream(q.device)
-    return a
+_NO_STRIDES = (0,) * 12
 
 
-def _attention_forward(q, k, v, lengths, scale, causal, with_lse):
+def _attention_forward(q, k, v, lengths, scale, causal, recorded):
     q, k, v = _rows16(q), _rows16(k), _rows16(v)
-    o = _token_major(*q.shape, q)
-    lse = torch.empty(q.shape[:3], dtype=torch.float32, device=q.device) if with_lse else None
-    _call("sofa_attention_forward", _attention_args(q, k, v, o, lse, lengths, scale, causal))
-    return q, k, v, o, lse
+    batch, heads, tokens, dim = q.shape
+    o, o_low, lse = _token_major(q), None, None
+    if recorded:
+        o_low, lse = _token_major(q), q.new_empty((batch, heads, tokens), dtype=torch.float32)
+    strides = (*q.stride()[:3], *k.stride()[:3], *v.stride()[:3], *o.stride()[:3])
+    device = q.device.index
+    _call("sofa_attention_forward", _ATTENTION.pack(
+        q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(), _ptr(o_low), _ptr(lse), _ptr(lengths),
+        0, 0, 0, 0, 0, _stream(device), *strides, *_NO_STRIDES, scale,
+        batch, heads, k.shape[1], tokens, dim, causal, device))
+    return q, k, v, o, o_low, lse
 
 
 class _Attention(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, v, lengths, scale, causal):
-        q, k, v, o, lse = _attention_forward(q, k, v, lengths, scale, causal, True)
-        ctx.save_for_backward(q, k, v, o, lse, lengths)
+        q, k, v, o, o_low, lse = _attention_forward(q, k, v, lengths, scale, causal, True)
+        ctx.save_for_backward(q, k, v, o, o_low, lse, lengths)
         ctx.scale, ctx.causal = scale, causal
         return o
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
+    @_once
     def backward(ctx, dout):
-        q, k, v, o, lse, lengths = ctx.saved_tensors
+        q, k, v, o, o_low, lse, lengths = ctx.saved_tensors
         dout = _rows16(dout)
         delta = torch.empty_like(lse)
-        dq = _token_major(*q.shape, q)
-        dk, dv = _token_major(*k.shape, k), _token_major(*v.shape, v)
-        a = _attention_args(q, k, v, o, lse, lengths, ctx.scale, ctx.causal)
-        a.dout, a.delta = dout.data_ptr(), delta.data_ptr()
-        a.dq, a.dk, a.dv = dq.data_ptr(), dk.data_ptr(), dv.data_ptr()
-        a.dout_stride[:], a.dq_stride[:] = dout.stride()[:3], dq.stride()[:3]
-        a.dk_stride[:], a.dv_stride[:] = dk.stride()[:3], dv.stride()[:3]
-        _call("sofa_attention_backward", a)
+        dq, dk, dv = _token_major(q), _token_major(k), _token_major(v)
+        batch, heads, tokens, dim = q.shape
+        device = q.device.index
+        _call("sofa_attention_backward", _ATTENTION.pack(
+            q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(), o_low.data_ptr(), lse.data_ptr(), _ptr(lengths),
+            dout.data_ptr(), delta.data_ptr(), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), _stream(device),
+            *q.stride()[:3], *k.stride()[:3], *v.stride()[:3], *o.stride()[:3],
+            *dout.stride()[:3], *dq.stride()[:3], *dk.stride()[:3], *dv.stride()[:3], ctx.scale,
+            batch, heads, k.shape[1], tokens, dim, ctx.causal, device))
         return dq, dk, dv, None, None, None
 
 
@@ -256,6 +238,9 @@ def _two_level(t: torch.Tensor, axes: int) -> Optional[Tuple[int, int, int]]:
     """(inner, outer_stride, inner_stride) such that element i of t's first `axes`
     axes is at i // inner * outer_stride + i % inner * inner_stride; None if two
     levels are not enough."""
+    if t.is_contiguous():
+        width = t.shape[-1] if axes < t.dim() else 1
+        return t.numel() // width, 0, width
     levels = []  # innermost first: [size, stride]
     for n, s in zip(reversed(t.shape[:axes]), reversed(t.stride()[:axes])):
         if n == 1:
@@ -292,39 +277,30 @@ def _logprob_split(rows: int, vocab: int) -> Tuple[int, int]:
     return -(-vocab // size), size
 
 
-def _logprob_args(logits, tokens, ignore_index, logprob, entropy, lse):
-    a = _LogprobArgs()
-    axes = logits.dim() - 1
-    a.rows, a.vocab = logprob.numel(), logits.shape[-1]
-    a.inner, a.outer_stride, a.inner_stride = _two_level(logits, axes)
-    tokens, a.token_outer_stride, a.token_inner_stride = _same_split(a.inner, a.rows, tokens, axes)
-    a.logits, a.tokens = logits.data_ptr(), tokens.data_ptr()
-    a.logprob, a.entropy, a.lse = logprob.data_ptr(), entropy.data_ptr(), lse.data_ptr()
-    a.ignore_index = ignore_index
-    a.parts, a.part_size = _logprob_split(a.rows, a.vocab)
-    a.type, a.device = _TYPES[logits.dtype], logits.device.index
-    a.stream = _stream(logits.device)
-    return a, tokens
-
-
 def _logprob_forward(logits, tokens, top, ignore_index):
-    if logits.stride(-1) != 1 or _two_level(logits, logits.dim() - 1) is None:
+    axes, rows, vocab = tokens.dim(), tokens.numel(), logits.shape[-1]
+    split = _two_level(logits, axes) if logits.stride(-1) == 1 else None
+    if split is None:
         logits = logits.contiguous()
-    device = logits.device
-    logprob, entropy, lse = (torch.empty(tokens.shape, dtype=torch.float32, device=device) for _ in range(3))
-    a, tokens = _logprob_args(logits, tokens, ignore_index, logprob, entropy, lse)
-    ids = values = None
+        split = rows, 0, vocab
+    tokens, *token_strides = _same_split(split[0], rows, tokens, axes)
+    shape = tokens.shape
+    logprob, entropy, lse = (logits.new_empty(shape, dtype=torch.float32) for _ in range(3))
+    parts, part_size = _logprob_split(rows, vocab)
+    ids = values = part_sums = part_top = None
     if top:
-        ids = torch.empty((*tokens.shape, top), dtype=torch.int64, device=device)
-        values = torch.empty((*tokens.shape, top), dtype=torch.float32, device=device)
-        a.top, a.top_ids, a.top_logprobs = top, ids.data_ptr(), values.data_ptr()
-    if a.parts > 1:
-        part_sums = torch.empty((a.rows, a.parts, 3), dtype=torch.float32, device=device)
-        a.part_sums = part_sums.data_ptr()
+        ids = tokens.new_empty((*shape, top))
+        values = logits.new_empty((*shape, top), dtype=torch.float32)
+    if parts > 1:
+        part_sums = logits.new_empty((rows, parts, 3), dtype=torch.float32)
         if top:
-            part_top = torch.empty((a.rows, a.parts, top), dtype=torch.int64, device=device)
-            a.part_top = part_top.data_ptr()
-    _call("sofa_logprob_forward", a)
+            part_top = tokens.new_empty((rows, parts, top))
+    device = logits.device.index
+    _call("sofa_logprob_forward", _LOGPROBS.pack(
+        logits.data_ptr(), tokens.data_ptr(), logprob.data_ptr(), entropy.data_ptr(), lse.data_ptr(),
+        _ptr(ids), _ptr(values), _ptr(part_sums), _ptr(part_top), 0, 0, 0, _stream(device),
+        rows, *split, 0, 0, 0, 0, *token_strides, ignore_index,
+        vocab, top, parts, part_size, _TYPES[logits.dtype], device))
     return logits, tokens, logprob, entropy, lse, ids, values
 
 
@@ -340,22 +316,27 @@ class _TokenLogprobs(torch.autograd.Function):
         return logprob, entropy, ids, values
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
+    @_once
     def backward(ctx, dlogprob, dentropy, _ids, _values):
         if dlogprob is None and dentropy is None:
             return None, None, None, None
         logits, tokens, entropy, lse = ctx.saved_tensors
-        dlogits = torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)
-        a, tokens = _logprob_args(logits, tokens, ctx.ignore_index, entropy, entropy, lse)
-        axes = tokens.dim()
+        axes, rows, vocab = tokens.dim(), tokens.numel(), logits.shape[-1]
+        split = _two_level(logits, axes)
+        tokens, *token_strides = _same_split(split[0], rows, tokens, axes)
+        strides = [0, 0, 0, 0]
         if dlogprob is not None:
-            dlogprob, a.grad_outer_stride, a.grad_inner_stride = _same_split(a.inner, a.rows, dlogprob, axes)
-            a.dlogprob = dlogprob.data_ptr()
+            dlogprob, *strides[:2] = _same_split(split[0], rows, dlogprob, axes)
         if dentropy is not None:
-            dentropy, a.grad2_outer_stride, a.grad2_inner_stride = _same_split(a.inner, a.rows, dentropy, axes)
-            a.dentropy = dentropy.data_ptr()
-        a.dlogits = dlogits.data_ptr()
-        _call("sofa_logprob_backward", a)
+            dentropy, *strides[2:] = _same_split(split[0], rows, dentropy, axes)
+        dlogits = torch.empty_like(logits, memory_format=torch.contiguous_format)
+        parts, part_size = _logprob_split(rows, vocab)
+        device = logits.device.index
+        _call("sofa_logprob_backward", _LOGPROBS.pack(
+            logits.data_ptr(), tokens.data_ptr(), entropy.data_ptr(), entropy.data_ptr(), lse.data_ptr(),
+            0, 0, 0, 0, _ptr(dlogprob), _ptr(dentropy), dlogits.data_ptr(), _stream(device),
+            rows, *split, *strides, *token_strides, ctx.ignore_index,
+            vocab, 0, parts, part_size, _TYPES[logits.dtype], device))
         return dlogits, None, None, None
 
 
@@ -407,33 +388,31 @@ def token_logprobs(
 
 
 # ------------------------------------------------------------------ residual norm
-def _dense(t: Optional[torch.Tensor]) -> Optional[torch.Tensor]:
-    return None if t is None else t.contiguous()
+def _norm_pack(pointers, x, branch_dtype, y_dtype, weight, post, gate, scale, eps, teams=0):
+    dim = x.shape[-1]
+    rows = x.numel() // dim
+    group_rows = rows if gate is None else rows * dim // gate.numel()
+    device = x.device.index
+    return _NORM.pack(
+        *pointers, _stream(device), rows, group_rows, eps, scale, dim,
+        _TYPES[x.dtype], _TYPES[branch_dtype], _TYPES[y_dtype], _TYPES[weight.dtype],
+        0 if post is None else _TYPES[post.dtype], 0 if gate is None else _TYPES[gate.dtype], teams, device)
 
 
-def _norm_args(x, branch, weight, post, gate, scale, eps, y_type):
-    a = _NormArgs()
-    a.x, a.branch, a.weight, a.post, a.gate = x.data_ptr(), _ptr(branch), weight.data_ptr(), _ptr(post), _ptr(gate)
-    a.dim = x.shape[-1]
-    a.rows = x.numel() // a.dim
-    a.group_rows = a.rows if gate is None else a.rows // (gate.numel() // a.dim)
-    a.eps, a.scale = eps, scale
-    a.x_type, a.y_type, a.weight_type = _TYPES[x.dtype], _TYPES[y_type], _TYPES[weight.dtype]
-    # without a branch the type only chooses a kernel, and one is built for it
-    a.branch_type = _TYPES[y_type if branch is None else branch.dtype]
-    a.post_type = 0 if post is None else _TYPES[post.dtype]
-    a.gate_type = 0 if gate is None else _TYPES[gate.dtype]
-    a.device = x.device.index
-    a.stream = _stream(x.device)
-    return a
+def _norm_teams(rows: int, groups: int, dim: int) -> int:
+    """Teams of the backward pass that share the rows of one gate.  About 512
+    workgroups fill the card twice; more would only add partial sums."""
+    return max(1, min((2048 if dim <= 1024 else 512) // groups, rows // groups))
 
 
 def _norm_forward(x, branch, weight, post, gate, scale, eps, out_dtype):
-    y = torch.empty(x.shape, dtype=out_dtype, device=x.device)
+    y = torch.empty_like(x, dtype=out_dtype)
     r = None if branch is None else torch.empty_like(x)
-    a = _norm_args(x, branch, weight, post, gate, scale, eps, out_dtype)
-    a.r, a.y = _ptr(r), y.data_ptr()
-    _call("sofa_norm_forward", a)
+    # without a branch its type only chooses a kernel, and one is built for y's
+    _call("sofa_norm_forward", _norm_pack(
+        (x.data_ptr(), _ptr(branch), weight.data_ptr(), _ptr(post), _ptr(gate), _ptr(r), y.data_ptr(),
+         0, 0, 0, 0, 0, 0, 0, 0),
+        x, out_dtype if branch is None else branch.dtype, out_dtype, weight, post, gate, scale, eps))
     return r, y
 
 
@@ -442,37 +421,39 @@ class _ResidualNorm(torch.autograd.Function):
     def forward(ctx, x, branch, weight, post, gate, scale, eps, out_dtype):
         r, y = _norm_forward(x, branch, weight, post, gate, scale, eps, out_dtype)
         ctx.set_materialize_grads(False)
-        uses_branch = post is not None or gate is not None
-        ctx.save_for_backward(x if r is None else r, branch if uses_branch else None, weight, post, gate)
-        ctx.scale, ctx.eps, ctx.out_dtype = scale, eps, out_dtype
-        ctx.branch_dtype = None if branch is None else branch.dtype
+        ctx.args = scale, eps, out_dtype, None if branch is None else branch.dtype
+        # a 32-bit sum is kept, one rounded to 16 bits is computed again
+        if branch is not None and x.dtype == torch.float32:
+            x = r
+            if post is None and gate is None:
+                branch = None
+        ctx.save_for_backward(x, branch, weight, post, gate)
         return r, y
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
+    @_once
     def backward(ctx, dr, dy):
         if dr is None and dy is None:
             return (None,) * 8
-        r, branch, weight, post, gate = ctx.saved_tensors
-        dr, dy = _dense(dr), _dense(dy)
-        a = _norm_args(r, branch, weight, post, gate, ctx.scale, ctx.eps, ctx.out_dtype)
-        if ctx.branch_dtype is not None:
-            a.branch_type = _TYPES[ctx.branch_dtype]
+        x, branch, weight, post, gate = ctx.saved_tensors
+        scale, eps, out_dtype, branch_dtype = ctx.args
+        dr, dy = dr if dr is None else dr.contiguous(), dy if dy is None else dy.contiguous()
         _, need_branch, need_weight, need_post, need_gate = ctx.needs_input_grad[:5]
-        dx = torch.empty_like(r)
-        dbranch = torch.empty(r.shape, dtype=ctx.branch_dtype, device=r.device) if need_branch else None
+        dx = torch.empty_like(x)
+        dbranch = torch.empty_like(x, dtype=branch_dtype) if need_branch else None
         dweight = torch.empty_like(weight) if need_weight else None
         dpost = torch.empty_like(post) if need_post else None
         dgate = torch.empty_like(gate) if need_gate else None
-        a.dr, a.dy, a.dx, a.dbranch = _ptr(dr), _ptr(dy), dx.data_ptr(), _ptr(dbranch)
-        a.dweight, a.dpost, a.dgate = _ptr(dweight), _ptr(dpost), _ptr(dgate)
-        sums = sum(t is not None for t in (dweight, dpost, dgate))
-        a.teams_per_group = _lib().sofa_norm_backward_teams(a.rows, a.group_rows, a.dim)
-        if sums:
-            partial = torch.empty(
-                (sums, a.rows // a.group_rows * a.teams_per_group, a.dim), dtype=torch.float32, device=r.device)
-            a.partial = partial.data_ptr()
-        _call("sofa_norm_backward", a)
+        dim = x.shape[-1]
+        groups = 1 if gate is None else gate.numel() // dim
+        teams = _norm_teams(x.numel() // dim, groups, dim)
+        sums = need_weight + need_post + need_gate
+        partial = x.new_empty((sums, groups * teams, dim), dtype=torch.float32) if sums else None
+        _call("sofa_norm_backward", _norm_pack(
+            (x.data_ptr(), _ptr(branch), weight.data_ptr(), _ptr(post), _ptr(gate), 0, 0,
+             _ptr(dr), _ptr(dy), dx.data_ptr(), _ptr(dbranch), _ptr(partial),
+             _ptr(dweight), _ptr(dpost), _ptr(dgate)),
+            x, branch_dtype or out_dtype, out_dtype, weight, post, gate, scale, eps, teams))
         return dx, dbranch, dweight, dpost, dgate, None, None, None
 
 
@@ -537,7 +518,8 @@ def residual_norm(
         for t in (branch, post_weight, gate):
             r = r if t is None else r * t.to(x.dtype)
         return (x if branch is None else r), (r * weight.to(x.dtype)).to(out_dtype)
-    args = (*(_dense(t) for t in (x, branch, weight, post_weight, gate)), float(scale), float(eps), out_dtype)
+    dense = (t if t is None or t.is_contiguous() else t.contiguous() for t in (x, branch, weight, post_weight, gate))
+    args = (*dense, float(scale), float(eps), out_dtype)
     if _recorded(x, branch, weight, post_weight, gate):
         r, y = _ResidualNorm.apply(*args)
     else:
