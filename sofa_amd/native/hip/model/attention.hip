@@ -42,13 +42,14 @@ struct AttentionArgs {
   const bf16* dout;
   float* delta;           // [batch][heads][tokens]
   bf16 *dq, *dk, *dv;
+  float* partial;         // [key_parts][2][batch][kv_heads][tokens][dim], or null
   void* stream;
   int64_t q_stride[3], k_stride[3], v_stride[3], o_stride[3];  // batch, head,
   int64_t dout_stride[3], dq_stride[3], dk_stride[3], dv_stride[3];  // token
   float scale;
-  int batch, heads, kv_heads, tokens, dim, causal, device;
+  int batch, heads, kv_heads, tokens, dim, causal, key_parts, device;
 };
-static_assert(sizeof(AttentionArgs) == 328, "as the caller packs it");
+static_assert(sizeof(AttentionArgs) == 344, "as the caller packs it");
 
 typedef bf16 bf16x4 __attribute__((ext_vector_type(4)));
 typedef bf16 bf16x8 __attribute__((ext_vector_type(8)));
@@ -60,50 +61,63 @@ constexpr int kThreads = 256;
 constexpr int kWaves = 4;
 constexpr int kRows = kWaves * 32;  // rows a workgroup owns
 constexpr int kTile = 64;           // rows of the other side at a time
+// between tokens, in elements: kTile rows are within 32-bit offsets
+constexpr int64_t kMaxStride = 1 << 24;
+constexpr int kMaxKeyParts = 8;
 
-// Where the 8 elements `chunk` of `row` of a tile are in LDS.  Rows are 256 or
-// 128 bytes, so that the same chunk of all rows falls on the same banks; the
-// exclusive or moves pairs of chunks such that 8 rows (a row read) as well as
-// 4 rows by 2 chunks (a transposed read) fall on different ones.
+// Where the 8 elements `chunk` of `row` of a tile are in LDS.  A row is 256 or
+// 128 bytes and the banks 256, so one chunk of all rows falls on the same banks;
+// the exclusive or moves it such that what one cycle pair reads is on different
+// ones: 16 rows of one chunk (a row operand), and 4 rows by 4 chunks (a column
+// operand).  Its lower two bits tell rows 4 apart, the next those 1 apart.
 template <int DP>
 __device__ __forceinline__ int swizzle(int row) {
-  return DP == 128 ? (row & 7) << 1 : ((row >> 1) & 3) << 1;
+  return DP == 128 ? (row & 3) << 2 | (row >> 2 & 3)
+                   : (row >> 1 & 1) << 2 | (row >> 2 & 3);
 }
 template <int DP>
 __device__ __forceinline__ int lds_at(int row, int chunk) {
   return row * DP + ((chunk ^ swizzle<DP>(row)) << 3);
 }
 
-// One thread's share of a tile of kTile rows on its way to LDS.  Rows behind
-// the last valid one repeat it, and chunks behind the last one repeat that:
-// what is computed from them is multiplied by zeros or not stored, and has
-// only to be finite.
+// Starts a tile of kTile rows on its way from memory to LDS, 16 bytes a lane
+// and past the registers: a wave's part of LDS is filled in the order of its
+// lanes, so each lane takes the chunk that belongs in its place.  `tile` is the
+// tile's first row, the same for the whole workgroup; addresses are then a
+// scalar base and one 32-bit offset.  Rows behind the last valid one repeat it,
+// and chunks behind the last one repeat that: what is computed from them is
+// multiplied by zeros or not stored, and has only to be finite.
 template <int DP>
-struct Staged {
-  static constexpr int kChunks = DP / 8;
-  static constexpr int kPasses = kTile * kChunks / kThreads;
-  bf16x8 x[kPasses];
+__device__ __forceinline__ void load_tile(const bf16* tile, int64_t stride,
+                                          int rows, int dim, bf16* to) {
+  typedef const __attribute__((address_space(1))) uint32_t* from_t;
+  typedef __attribute__((address_space(3))) uint32_t* to_t;
+  constexpr int kChunks = DP / 8;
+  constexpr int kStep = kThreads / kChunks;  // rows a pass
+  const uint32_t row = threadIdx.x / kChunks;
+  const int chunk = threadIdx.x % kChunks ^ swizzle<DP>(row);
+  const uint32_t at = min(chunk, dim / 8 - 1) * 8;
+  const uint32_t step = (uint32_t) stride;  // up to kMaxStride
+  to += __builtin_amdgcn_readfirstlane(threadIdx.x / kWave) * kWave * 8;
+#pragma unroll
+  for (int p = 0; p < kTile / kStep; ++p) {
+    // swizzle() repeats after 16 rows, so that the chunk is the same each pass
+    const bf16* from =
+        rows >= kTile
+            ? tile + p * kStep * stride + (row * step + at)
+            : tile + (min(row + p * kStep, (uint32_t) rows - 1) * step + at);
+    __builtin_amdgcn_global_load_lds((from_t) from, (to_t) (to + p * kStep * DP),
+                                     16, 0, 0);
+  }
+}
 
-  __device__ __forceinline__ void load(const bf16* base, int64_t stride,
-                                       int first, int rows, int dim) {
-    const int chunk = min((int) threadIdx.x % kChunks, dim / 8 - 1);
-#pragma unroll
-    for (int p = 0; p < kPasses; ++p) {
-      const int row =
-          first + p * (kThreads / kChunks) + (int) threadIdx.x / kChunks;
-      x[p] = *reinterpret_cast<const bf16x8*>(
-          base + (int64_t) min(row, rows - 1) * stride + chunk * 8);
-    }
-  }
-  __device__ __forceinline__ void store(bf16* tile) const {
-    const int chunk = threadIdx.x % kChunks;
-#pragma unroll
-    for (int p = 0; p < kPasses; ++p) {
-      const int row = p * (kThreads / kChunks) + threadIdx.x / kChunks;
-      *reinterpret_cast<bf16x8*>(tile + lds_at<DP>(row, chunk)) = x[p];
-    }
-  }
-};
+// All of the workgroup's tiles on their way are there.  Reads of LDS wait for
+// this wave's own loads before that: the next ones start where no more reads
+// follow for some time, after the scores' products.
+__device__ __forceinline__ void arrived() {
+  __builtin_amdgcn_s_waitcnt(0x0f70);  // vmcnt(0)
+  __syncthreads();
+}
 
 // A operand: rows first..first+31 of a tile, elements 16 s..16 s + 15
 template <int DP>
@@ -189,6 +203,24 @@ __device__ __forceinline__ void store_row(bf16* row,
     }
 }
 
+// The same in 32 bits
+template <int DP>
+__device__ __forceinline__ void store_row(float* row,
+                                          const floatx16 (&acc)[DP / 32],
+                                          bool valid, int dim) {
+  const int h = threadIdx.x % kWave / 32;
+#pragma unroll
+  for (int b = 0; b < DP / 32; ++b)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int at = b * 32 + i * 8 + h * 4;
+      floatx4 x;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) x[j] = valid ? acc[b][i * 4 + j] : 0.f;
+      if (at < dim) *reinterpret_cast<floatx4*>(row + at) = x;
+    }
+}
+
 __device__ __forceinline__ float other_half(float x) {
   return __shfl_xor(x, 32);
 }
@@ -211,8 +243,8 @@ __device__ __forceinline__ int valid_tokens(const AttentionArgs& a, int batch) {
 template <int DP, bool CAUSAL>
 __global__ __launch_bounds__(kThreads, 2) void attention_forward_kernel(
     AttentionArgs a) {
-  __shared__ __align__(16) bf16 k_tile[kTile * DP];
-  __shared__ __align__(16) bf16 v_tile[kTile * DP];
+  __shared__ __align__(16) bf16 k_tiles[2][kTile * DP];
+  __shared__ __align__(16) bf16 v_tiles[2][kTile * DP];
   const int blocks = (a.tokens + kRows - 1) / kRows;
   int bh, block;
   whose(a.batch * a.heads, blocks, CAUSAL, bh, block);
@@ -237,39 +269,44 @@ __global__ __launch_bounds__(kThreads, 2) void attention_forward_kernel(
 
   int end = block * kRows < n ? n : 0;
   if (CAUSAL) end = min(end, (block + 1) * kRows);
-  for (int first = 0; first < end; first += kTile) {
-    Staged<DP> ks, vs;
-    ks.load(k, a.k_stride[2], first, n, a.dim);
-    vs.load(v, a.v_stride[2], first, n, a.dim);
-    __syncthreads();
-    ks.store(k_tile);
-    vs.store(v_tile);
-    __syncthreads();
-    if (CAUSAL && first > wave_row + 31) continue;
-
+  auto load = [&](int first, int buffer) {
+    if (first >= end) return;
+    load_tile<DP>(k + first * a.k_stride[2], a.k_stride[2], n - first, a.dim,
+                  k_tiles[buffer]);
+    load_tile<DP>(v + first * a.v_stride[2], a.v_stride[2], n - first, a.dim,
+                  v_tiles[buffer]);
+  };
+  auto tile = [&]<bool MASKED>(int first, int buffer) {
+    const bf16 *k_tile = k_tiles[buffer], *v_tile = v_tiles[buffer];
     floatx16 s[2] = {};
 #pragma unroll
     for (int d = 0; d < DP / 16; ++d)
 #pragma unroll
       for (int b = 0; b < 2; ++b)
         s[b] = mfma(row_operand<DP>(k_tile, b * 32, d), q[d], s[b]);
-    if (first + kTile > n || (CAUSAL && first + kTile - 1 > wave_row)) {
+    load(first + kTile, buffer ^ 1);
+    if (MASKED) {
 #pragma unroll
-      for (int b = 0; b < 2; ++b)
-#pragma unroll
-        for (int i = 0; i < 16; ++i) {
-          const int key = first + b * 32 + i / 4 * 8 + h * 4 + i % 4;
-          if (key >= n || (CAUSAL && key > row)) s[b][i] = -INFINITY;
-        }
+      for (int i = 0; i < 32; ++i) {
+        const int key = first + i / 4 * 8 + h * 4 + i % 4;
+        if (key >= n || (CAUSAL && key > row)) s[i / 16][i % 16] = -INFINITY;
+      }
     }
     float most = s[0][0];
 #pragma unroll
     for (int i = 1; i < 32; ++i) most = fmaxf(most, s[i / 16][i % 16]);
     most = fmaxf(most, other_half(most));
-    // the first tile holds key 0, which every row sees: m is finite after it
-    const float next = fmaxf(m, most * scale);
-    const float fade = exp2_fast(m - next);
-    m = next;
+    // m follows the maximum in steps of 2^8 or more: the probabilities are
+    // relative to it anyway, and most tiles need no new factor for the sums.
+    // The first tile holds key 0, which every row sees: m is finite after it.
+    if (__any(most * scale > m + 8.f)) {
+      const float next = fmaxf(m, most * scale);
+      const float fade = exp2_fast(m - next);
+      m = next;
+      l *= fade;
+#pragma unroll
+      for (int b = 0; b < DP / 32; ++b) acc[b] *= fade;
+    }
     float sum = 0.f;
 #pragma unroll
     for (int i = 0; i < 32; ++i) {
@@ -277,9 +314,7 @@ __global__ __launch_bounds__(kThreads, 2) void attention_forward_kernel(
       s[i / 16][i % 16] = p;
       sum += p;
     }
-    l = l * fade + sum;
-#pragma unroll
-    for (int b = 0; b < DP / 32; ++b) acc[b] *= fade;
+    l += sum;
 #pragma unroll
     for (int p = 0; p < 4; ++p) {
       const bf16x8 prob = rounded(s[p / 2], p % 2);
@@ -287,6 +322,21 @@ __global__ __launch_bounds__(kThreads, 2) void attention_forward_kernel(
       for (int b = 0; b < DP / 32; ++b)
         acc[b] = mfma(column_operand<DP>(v_tile, p * 16, b), prob, acc[b]);
     }
+  };
+  // tiles that every row sees whole, then the others
+  const int whole = (CAUSAL ? min(block * kRows, n) : n) / kTile * kTile;
+  int first = 0, buffer = 0;
+  load(0, 0);
+  for (; first < min(whole, end); first += kTile, buffer ^= 1) {
+    arrived();
+    tile.template operator()<false>(first, buffer);
+  }
+  for (; first < end; first += kTile, buffer ^= 1) {
+    arrived();
+    if (CAUSAL && first > wave_row + 31)
+      load(first + kTile, buffer ^ 1);
+    else
+      tile.template operator()<true>(first, buffer);
   }
 
   if (row >= a.tokens) return;
@@ -305,8 +355,8 @@ __global__ __launch_bounds__(kThreads, 2) void attention_forward_kernel(
 template <int DP, bool CAUSAL>
 __global__ __launch_bounds__(kThreads, 2) void attention_dq_kernel(
     AttentionArgs a) {
-  __shared__ __align__(16) bf16 k_tile[kTile * DP];
-  __shared__ __align__(16) bf16 v_tile[kTile * DP];
+  __shared__ __align__(16) bf16 k_tiles[2][kTile * DP];
+  __shared__ __align__(16) bf16 v_tiles[2][kTile * DP];
   const int blocks = (a.tokens + kRows - 1) / kRows;
   int bh, block;
   whose(a.batch * a.heads, blocks, CAUSAL, bh, block);
@@ -353,44 +403,62 @@ __global__ __launch_bounds__(kThreads, 2) void attention_dq_kernel(
 
   int end = block * kRows < n ? n : 0;
   if (CAUSAL) end = min(end, (block + 1) * kRows);
-  for (int first = 0; first < end; first += kTile) {
-    Staged<DP> ks, vs;
-    ks.load(k, a.k_stride[2], first, n, a.dim);
-    vs.load(v, a.v_stride[2], first, n, a.dim);
-    __syncthreads();
-    ks.store(k_tile);
-    vs.store(v_tile);
-    __syncthreads();
-    if (CAUSAL && first > wave_row + 31) continue;
-
-    const bool masked = first + kTile > n ||
-                        (CAUSAL && first + kTile - 1 > wave_row);
+  auto load = [&](int first, int buffer) {
+    if (first >= end) return;
+    load_tile<DP>(k + first * a.k_stride[2], a.k_stride[2], n - first, a.dim,
+                  k_tiles[buffer]);
+    load_tile<DP>(v + first * a.v_stride[2], a.v_stride[2], n - first, a.dim,
+                  v_tiles[buffer]);
+  };
+  // 32 BLOCKS keys at a time
+  constexpr int kBlocks = DP <= 64 ? 1 : 2;
+  auto tile = [&]<bool MASKED>(int first, int buffer) {
+    const bf16 *k_tile = k_tiles[buffer], *v_tile = v_tiles[buffer];
 #pragma unroll
-    for (int b = 0; b < 2; ++b) {
-      floatx16 s = {}, dp = {};
+    for (int part = 0; part < 2 / kBlocks; ++part) {
+      floatx16 s[kBlocks] = {}, dp[kBlocks] = {};
+      const int line = part * kBlocks * 32;
 #pragma unroll
-      for (int d = 0; d < DP / 16; ++d) {
-        s = mfma(row_operand<DP>(k_tile, b * 32, d), q[d], s);
-        dp = mfma(row_operand<DP>(v_tile, b * 32, d), dout[d], dp);
-      }
+      for (int d = 0; d < DP / 16; ++d)
 #pragma unroll
-      for (int i = 0; i < 16; ++i) {
-        float p = exp2_fast(s[i] * scale - lse);
-        if (masked) {
-          const int key = first + b * 32 + i / 4 * 8 + h * 4 + i % 4;
+        for (int b = 0; b < kBlocks; ++b) {
+          s[b] = mfma(row_operand<DP>(k_tile, line + b * 32, d), q[d], s[b]);
+          dp[b] =
+              mfma(row_operand<DP>(v_tile, line + b * 32, d), dout[d], dp[b]);
+        }
+      if (part == 2 / kBlocks - 1) load(first + kTile, buffer ^ 1);
+#pragma unroll
+      for (int i = 0; i < 16 * kBlocks; ++i) {
+        float p = exp2_fast(s[i / 16][i % 16] * scale - lse);
+        if (MASKED) {
+          const int key = first + line + i / 4 * 8 + h * 4 + i % 4;
           if (key >= n || (CAUSAL && key > row)) p = 0.f;
         }
-        s[i] = p * (dp[i] - delta);
+        s[i / 16][i % 16] = p * (dp[i / 16][i % 16] - delta);
       }
 #pragma unroll
-      for (int p = 0; p < 2; ++p) {
-        const bf16x8 ds = rounded(s, p);
+      for (int p = 0; p < 2 * kBlocks; ++p) {
+        const bf16x8 ds = rounded(s[p / 2], p % 2);
 #pragma unroll
         for (int c = 0; c < DP / 32; ++c)
-          acc[c] =
-              mfma(column_operand<DP>(k_tile, b * 32 + p * 16, c), ds, acc[c]);
+          acc[c] = mfma(column_operand<DP>(k_tile, line + p * 16, c), ds, acc[c]);
       }
     }
+  };
+  // tiles that every row sees whole, then the others
+  const int whole = (CAUSAL ? min(block * kRows, n) : n) / kTile * kTile;
+  int first = 0, buffer = 0;
+  load(0, 0);
+  for (; first < min(whole, end); first += kTile, buffer ^= 1) {
+    arrived();
+    tile.template operator()<false>(first, buffer);
+  }
+  for (; first < end; first += kTile, buffer ^= 1) {
+    arrived();
+    if (CAUSAL && first > wave_row + 31)
+      load(first + kTile, buffer ^ 1);
+    else
+      tile.template operator()<true>(first, buffer);
   }
   if (row >= a.tokens) return;
   store_row<DP>(a.dq + batch * a.dq_stride[0] + head * a.dq_stride[1] +
@@ -398,16 +466,22 @@ __global__ __launch_bounds__(kThreads, 2) void attention_dq_kernel(
                 acc, a.scale, valid, a.dim);
 }
 
-// dK and dV, summed over the heads that share them
+// dK and dV, summed over the heads that share them.  A workgroup takes its
+// share, one of key_parts, of the tiles of these heads' rows.
 template <int DP, bool CAUSAL>
-__global__ __launch_bounds__(kThreads, 1) void attention_dkv_kernel(
-    AttentionArgs a) {
-  __shared__ __align__(16) bf16 q_tile[kTile * DP];
-  __shared__ __align__(16) bf16 do_tile[kTile * DP];
-  __shared__ __align__(16) float lse_tile[kTile], delta_tile[kTile];
+__global__ __launch_bounds__(kThreads, DP <= 64 ? 2 : 1) void
+attention_dkv_kernel(AttentionArgs a) {
+  __shared__ __align__(16) bf16 q_tiles[2][kTile * DP];
+  __shared__ __align__(16) bf16 do_tiles[2][kTile * DP];
+  // what the products of a row start from: -lse in units of the scores, and
+  // -delta
+  __shared__ __align__(16) float lse_tiles[2][kTile];
+  __shared__ __align__(16) float delta_tiles[2][kTile];
   const int blocks = (a.tokens + kRows - 1) / kRows;
   int bh, block;
-  whose(a.batch * a.kv_heads, blocks, false, bh, block);
+  whose(a.batch * a.kv_heads, blocks * a.key_parts, false, bh, block);
+  const int part = block % a.key_parts;
+  block /= a.key_parts;
   const int batch = bh / a.kv_heads, kv_head = bh % a.kv_heads;
   const int group = a.heads / a.kv_heads;
   const int lane = threadIdx.x % kWave, wave = threadIdx.x / kWave;
@@ -429,76 +503,150 @@ __global__ __launch_bounds__(kThreads, 1) void attention_dkv_kernel(
   floatx16 dk[DP / 32] = {}, dv[DP / 32] = {};
   const float scale = a.scale * kLog2e;
 
-  const int end = block * kRows < n ? n : 0;
+  // the tiles of one head after those of the other; in each from the last
+  // rows to the first, so that workgroups of other keys, which start at other
+  // rows where the mask is causal, read the same tiles at the same time
   const int start = CAUSAL ? block * kRows : 0;  // a multiple of kTile
-  for (int g = 0; g < group; ++g) {
-    const int head = kv_head * group + g;
-    const bf16* q = a.q + batch * a.q_stride[0] + head * a.q_stride[1];
-    const bf16* dout =
-        a.dout + batch * a.dout_stride[0] + head * a.dout_stride[1];
-    const int64_t stats = ((int64_t) batch * a.heads + head) * a.tokens;
-    for (int first = start; first < end; first += kTile) {
-      Staged<DP> qs, dos;
-      qs.load(q, a.q_stride[2], first, n, a.dim);
-      dos.load(dout, a.dout_stride[2], first, n, a.dim);
-      float lse = INFINITY, delta = 0.f;
-      if (threadIdx.x < kTile && first + (int) threadIdx.x < n) {
-        lse = a.lse[stats + first + threadIdx.x];
-        delta = a.delta[stats + first + threadIdx.x];
-      }
-      __syncthreads();
-      qs.store(q_tile);
-      dos.store(do_tile);
-      if (threadIdx.x < kTile) {
-        lse_tile[threadIdx.x] = lse;
-        delta_tile[threadIdx.x] = delta;
-      }
-      __syncthreads();
-      if (CAUSAL && first + kTile - 1 < wave_key) continue;
-
-      const bool masked = CAUSAL && first < wave_key + 31;
+  const int tiles = block * kRows < n ? (n - start + kTile - 1) / kTile : 0;
+  const int masked = CAUSAL ? min(tiles, kRows / kTile) : 0;  // the last ones
+  int step = (int) ((int64_t) tiles * group * part / a.key_parts);
+  const int stop = (int) ((int64_t) tiles * group * (part + 1) / a.key_parts);
+  float lse = 0.f, delta = 0.f;
+  auto load = [&](int step, int buffer) {
+    if (step >= stop) return;
+    const int head = kv_head * group + step / tiles;
+    const int first = start + (tiles - 1 - step % tiles) * kTile;
+    load_tile<DP>(a.q + batch * a.q_stride[0] + head * a.q_stride[1] +
+                      first * a.q_stride[2],
+                  a.q_stride[2], n - first, a.dim, q_tiles[buffer]);
+    load_tile<DP>(a.dout + batch * a.dout_stride[0] + head * a.dout_stride[1] +
+                      first * a.dout_stride[2],
+                  a.dout_stride[2], n - first, a.dim, do_tiles[buffer]);
+    // +inf makes every probability of a row that is not there 0
+    lse = INFINITY;
+    delta = 0.f;
+    if (threadIdx.x < kTile && first + (int) threadIdx.x < n) {
+      const int64_t at = ((int64_t) batch * a.heads + head) * a.tokens + first +
+                         threadIdx.x;
+      lse = a.lse[at];
+      delta = a.delta[at];
+    }
+  };
+  const float inv_scale = 1.f / scale;
+  auto store = [&](int buffer) {
+    if (threadIdx.x < kTile) {
+      lse_tiles[buffer][threadIdx.x] = -lse * inv_scale;
+      delta_tiles[buffer][threadIdx.x] = -delta;
+    }
+  };
+  auto tile = [&]<bool MASKED>(int step, int buffer) {
+    const bf16 *q_tile = q_tiles[buffer], *do_tile = do_tiles[buffer];
+    floatx16 s[2], dp[2];
 #pragma unroll
-      for (int b = 0; b < 2; ++b) {
-        floatx16 s = {}, dp = {};
+    for (int i = 0; i < 8; ++i) {
+      const int line = i * 8 + h * 4;
+      const floatx4 x =
+          *reinterpret_cast<const floatx4*>(lse_tiles[buffer] + line);
+      const floatx4 y =
+          *reinterpret_cast<const floatx4*>(delta_tiles[buffer] + line);
 #pragma unroll
-        for (int d = 0; d < DP / 16; ++d) {
-          s = mfma(row_operand<DP>(q_tile, b * 32, d), k[d], s);
-          dp = mfma(row_operand<DP>(do_tile, b * 32, d), v[d], dp);
-        }
-        floatx16 prob;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const int line = b * 32 + i * 8 + h * 4;
-          const floatx4 lses = *reinterpret_cast<floatx4*>(lse_tile + line);
-          const floatx4 deltas = *reinterpret_cast<floatx4*>(delta_tile + line);
-#pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            float p = exp2_fast(s[i * 4 + j] * scale - lses[j]);
-            if (masked && key > first + line + j) p = 0.f;
-            prob[i * 4 + j] = p;
-            s[i * 4 + j] = p * (dp[i * 4 + j] - deltas[j]);
-          }
-        }
-#pragma unroll
-        for (int p = 0; p < 2; ++p) {
-          const bf16x8 probs = rounded(prob, p), ds = rounded(s, p);
-#pragma unroll
-          for (int c = 0; c < DP / 32; ++c) {
-            const int line = b * 32 + p * 16;
-            dv[c] = mfma(column_operand<DP>(do_tile, line, c), probs, dv[c]);
-            dk[c] = mfma(column_operand<DP>(q_tile, line, c), ds, dk[c]);
-          }
-        }
+      for (int j = 0; j < 4; ++j) {
+        s[i / 4][i % 4 * 4 + j] = x[j];
+        dp[i / 4][i % 4 * 4 + j] = y[j];
       }
     }
+#pragma unroll
+    for (int d = 0; d < DP / 16; ++d)
+#pragma unroll
+      for (int b = 0; b < 2; ++b) {
+        s[b] = mfma(row_operand<DP>(q_tile, b * 32, d), k[d], s[b]);
+        dp[b] = mfma(row_operand<DP>(do_tile, b * 32, d), v[d], dp[b]);
+      }
+    load(step + 1, buffer ^ 1);
+    const int first = start + (tiles - 1 - step % tiles) * kTile;
+#pragma unroll
+    for (int i = 0; i < 32; ++i) {
+      float p = exp2_fast(s[i / 16][i % 16] * scale);
+      if (MASKED && key > first + i / 4 * 8 + h * 4 + i % 4) p = 0.f;
+      s[i / 16][i % 16] = p;
+      dp[i / 16][i % 16] *= p;
+    }
+#pragma unroll
+    for (int p = 0; p < 4; ++p) {
+      const bf16x8 probs = rounded(s[p / 2], p % 2);
+      const bf16x8 ds = rounded(dp[p / 2], p % 2);
+#pragma unroll
+      for (int c = 0; c < DP / 32; ++c) {
+        dv[c] = mfma(column_operand<DP>(do_tile, p * 16, c), probs, dv[c]);
+        dk[c] = mfma(column_operand<DP>(q_tile, p * 16, c), ds, dk[c]);
+      }
+    }
+  };
+  int buffer = 0;
+  load(step, 0);
+  store(0);
+  while (step < stop) {
+    // tiles whose rows all see every key, then those of the mask's edge
+    int until = min(stop, step - step % tiles + tiles - masked);
+    for (; step < until; ++step, buffer ^= 1) {
+      arrived();
+      tile.template operator()<false>(step, buffer);
+      store(buffer ^ 1);
+    }
+    if (!CAUSAL) continue;
+    until = min(stop, step - step % tiles + tiles);
+    if (step % tiles < tiles - masked) until = step;
+    for (; step < until; ++step, buffer ^= 1) {
+      arrived();
+      const int first = start + (tiles - 1 - step % tiles) * kTile;
+      if (first + kTile - 1 < wave_key)
+        load(step + 1, buffer ^ 1);
+      else
+        tile.template operator()<true>(step, buffer);
+      store(buffer ^ 1);
+    }
   }
+
   if (key >= a.tokens) return;
+  if (a.key_parts > 1) {
+    const int64_t size = (int64_t) a.batch * a.kv_heads * a.tokens * a.dim;
+    float* out = a.partial + part * 2 * size +
+                 ((int64_t) bh * a.tokens + key) * a.dim;
+    store_row<DP>(out, dk, valid, a.dim);
+    store_row<DP>(out + size, dv, valid, a.dim);
+    return;
+  }
   store_row<DP>(a.dk + batch * a.dk_stride[0] + kv_head * a.dk_stride[1] +
                     (int64_t) key * a.dk_stride[2],
                 dk, a.scale, valid, a.dim);
   store_row<DP>(a.dv + batch * a.dv_stride[0] + kv_head * a.dv_stride[1] +
                     (int64_t) key * a.dv_stride[2],
                 dv, 1.f, valid, a.dim);
+}
+
+// dK and dV as the sum of their parts, in order; 8 elements a thread
+__global__ __launch_bounds__(kThreads) void attention_join_kernel(
+    AttentionArgs a) {
+  const int64_t size = (int64_t) a.batch * a.kv_heads * a.tokens * a.dim;
+  const int64_t at = ((int64_t) blockIdx.x * kThreads + threadIdx.x) * 8;
+  if (at >= 2 * size) return;
+  const bool is_v = at >= size;
+  float sum[8] = {};
+  for (int part = 0; part < a.key_parts; ++part) {
+    float x[8];
+    load8(a.partial + part * 2 * size + at, x);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) sum[j] += x[j];
+  }
+#pragma unroll
+  for (int j = 0; j < 8; ++j) sum[j] *= is_v ? 1.f : a.scale;
+  const int64_t row = (is_v ? at - size : at) / a.dim;
+  const int64_t token = row % a.tokens, head = row / a.tokens % a.kv_heads;
+  const int64_t batch = row / a.tokens / a.kv_heads;
+  const int64_t* stride = is_v ? a.dv_stride : a.dk_stride;
+  store8((is_v ? a.dv : a.dk) + batch * stride[0] + head * stride[1] +
+             token * stride[2] + at % a.dim,
+         sum);
 }
 
 template <int DP, bool CAUSAL>
@@ -519,7 +667,15 @@ int backward(const AttentionArgs& a) {
   int status = (int) hipGetLastError();
   if (status) return status;
   hipLaunchKernelGGL((attention_dkv_kernel<DP, CAUSAL>),
-                     dim3((unsigned) (blocks * a.batch * a.kv_heads)),
+                     dim3((unsigned) (blocks * a.batch * a.kv_heads *
+                                      a.key_parts)),
+                     dim3(kThreads), 0, static_cast<hipStream_t>(a.stream), a);
+  status = (int) hipGetLastError();
+  if (status || a.key_parts == 1) return status;
+  const int64_t threads =
+      (int64_t) a.batch * a.kv_heads * a.tokens * (a.dim / 8) * 2;
+  hipLaunchKernelGGL(attention_join_kernel,
+                     dim3((unsigned) ((threads + kThreads - 1) / kThreads)),
                      dim3(kThreads), 0, static_cast<hipStream_t>(a.stream), a);
   return (int) hipGetLastError();
 }
@@ -529,10 +685,12 @@ bool sound(const AttentionArgs* a) {
       a->heads % a->kv_heads || a->tokens <= 0 || a->dim <= 0 || a->dim % 8 ||
       a->dim > 128 || !a->q || !a->k || !a->v || !a->o)
     return false;
+  for (const int64_t* stride : {a->q_stride, a->k_stride, a->v_stride})
+    if (stride[2] < 0 || stride[2] > kMaxStride) return false;
   // the grid, and row numbers up to the end of a block
   return a->tokens <= (1 << 24) &&
          (int64_t) a->batch * a->heads * ((a->tokens + kRows - 1) / kRows) <=
-             INT32_MAX;
+             INT32_MAX / kMaxKeyParts;
 }
 
 }  // namespace
@@ -553,7 +711,8 @@ int sofa_attention_forward(const sofa_model::AttentionArgs* a) {
 int sofa_attention_backward(const sofa_model::AttentionArgs* a) {
   using namespace sofa_model;
   if (!sound(a) || !a->dout || !a->o_low || !a->lse || !a->delta || !a->dq || !a->dk ||
-      !a->dv)
+      !a->dv || a->key_parts < 1 || a->key_parts > kMaxKeyParts ||
+      (a->key_parts > 1 && !a->partial) || a->dout_stride[2] < 0 || a->dout_stride[2] > kMaxStride)
     return kBadArgument;
   DeviceGuard guard(a->device);
   if (guard.status()) return guard.status();

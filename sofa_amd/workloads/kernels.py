@@ -29,13 +29,14 @@ _TYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
 MAX_HEAD_DIM = 128
 MAX_TOKENS = 1 << 24
 MAX_TOP = 32
+_MAX_TOKEN_STRIDE = 1 << 24  # elements
 MAX_NORM_DIM = 16384
 MAX_VOCAB = 1 << 30
 
 # The argument structures of the C entries, packed in one call each: pointers,
 # then 64-bit, 32-bit floating and 32-bit whole numbers, in the order of their
 # declarations in native/hip/model.  "0q" pads the end as C does.
-_ATTENTION = struct.Struct("13P24qf7i0q")
+_ATTENTION = struct.Struct("14P24qf8i0q")
 _LOGPROBS = struct.Struct("13P11q6i0q")
 _NORM = struct.Struct("16P2q2f9i0q")
 
@@ -100,11 +101,10 @@ def _recorded(*tensors: Optional[torch.Tensor]) -> bool:
 
 # ------------------------------------------------------------------ attention
 def _rows16(t: torch.Tensor) -> torch.Tensor:
-    """t, or a copy, with dense rows that start at multiples of 16 bytes."""
+    """t, or a copy, with dense rows that start at multiples of 16 bytes and are
+    not further apart than the kernels' offsets within a tile reach."""
     a, b, c, dense = t.stride()
-    # the stride of an axis of one is never used
-    if dense == 1 and t.data_ptr() % 16 == 0 and (
-            (a | b | c) % 8 == 0 or all(s % 8 == 0 or n == 1 for s, n in zip((a, b, c), t.shape))):
+    if dense == 1 and c <= _MAX_TOKEN_STRIDE and t.data_ptr() % 16 == 0 and (a | b | c) % 8 == 0:
         return t
     return t.clone(memory_format=torch.contiguous_format)
 
@@ -129,9 +129,17 @@ def _attention_forward(q, k, v, lengths, scale, causal, recorded):
     device = q.device.index
     _call("sofa_attention_forward", _ATTENTION.pack(
         q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(), _ptr(o_low), _ptr(lse), _ptr(lengths),
-        0, 0, 0, 0, 0, _stream(device), *strides, *_NO_STRIDES, scale,
-        batch, heads, k.shape[1], tokens, dim, causal, device))
+        0, 0, 0, 0, 0, 0, _stream(device), *strides, *_NO_STRIDES, scale,
+        batch, heads, k.shape[1], tokens, dim, causal, 1, device))
     return q, k, v, o, o_low, lse
+
+
+def _key_parts(batch: int, heads: int, kv_heads: int, tokens: int, dim: int, causal: bool) -> int:
+    """Workgroups that share the rows behind one block of 128 keys."""
+    groups = batch * kv_heads * -(-tokens // 128)
+    wanted = (256 if dim > 64 else 512) * (2 if causal else 1)
+    steps = -(-tokens // 64) * (heads // kv_heads) // (2 if causal else 1)
+    return max(1, min(8, -(-wanted // groups), steps // 4))
 
 
 class _Attention(torch.autograd.Function):
@@ -150,13 +158,16 @@ class _Attention(torch.autograd.Function):
         delta = torch.empty_like(lse)
         dq, dk, dv = _token_major(q), _token_major(k), _token_major(v)
         batch, heads, tokens, dim = q.shape
-        device = q.device.index
+        kv_heads, device = k.shape[1], q.device.index
+        parts = _key_parts(batch, heads, kv_heads, tokens, dim, ctx.causal)
+        partial = q.new_empty((parts, 2, *k.shape), dtype=torch.float32) if parts > 1 else None
         _call("sofa_attention_backward", _ATTENTION.pack(
             q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(), o_low.data_ptr(), lse.data_ptr(), _ptr(lengths),
-            dout.data_ptr(), delta.data_ptr(), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), _stream(device),
+            dout.data_ptr(), delta.data_ptr(), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(),
+            _ptr(partial), _stream(device),
             *q.stride()[:3], *k.stride()[:3], *v.stride()[:3], *o.stride()[:3],
             *dout.stride()[:3], *dq.stride()[:3], *dk.stride()[:3], *dv.stride()[:3], ctx.scale,
-            batch, heads, k.shape[1], tokens, dim, ctx.causal, device))
+            batch, heads, kv_heads, tokens, dim, ctx.causal, parts, device))
         return dq, dk, dv, None, None, None
 
 
