@@ -13,8 +13,9 @@
 // registers.  A row belongs to a team of one wave (short rows) or one
 // workgroup, 8 VPT elements a thread, so the statistics take one reduction
 // each.  Sums over rows (dweight, dpost, dgate) stay in registers over the
-// team's rows, go to one partial row per team and are added in a fixed order
-// by a second kernel: no atomics, the same bits every time.
+// team's rows, are joined in LDS, go to one partial row per workgroup and are
+// added in a fixed order by a second kernel: no atomics, the same bits every
+// time.
 
 #include "model_ops.h"
 
@@ -26,13 +27,13 @@ struct NormArgs {
   void *r, *y;                                    // r: null without a branch
   const void *dr, *dy;                            // either may be null
   void *dx, *dbranch;                             // dbranch: or null
-  float* partial;  // [sums][teams][dim]: dweight, then dpost, then dgate
+  float* partial;  // [sums][workgroups][dim]: dweight, then dpost, then dgate
   void *dweight, *dpost, *dgate;                  // each or null
   void* stream;
   int64_t rows, group_rows;  // rows, and rows that share one gate
   float eps, scale;
   int dim, x_type, branch_type, y_type, weight_type, post_type, gate_type;
-  int teams_per_group;       // backward: teams that share a gate's rows
+  int group_blocks;          // backward: workgroups that share a gate's rows
   int device;
 };
 static_assert(sizeof(NormArgs) == 192, "as the caller packs it");
@@ -150,8 +151,8 @@ __global__ __launch_bounds__(kBlock<TEAM>) void norm_forward_kernel(
   }
 }
 
-// A team takes consecutive rows of one gate's group, so that the gate and its
-// gradient stay in registers too.
+// A workgroup takes consecutive rows of one gate's group, so that the gate and
+// its gradient stay in registers too; its teams take them in turn.
 // EXTRA: the branch has a norm or a gate; without them their registers
 // (5 of 8 vectors) are not held.  x is r where that is held in 32 bits (or there
 // is no branch); a 16-bit r has lost what the gradients of the weights need,
@@ -161,17 +162,11 @@ __global__ __launch_bounds__(kBlock<TEAM>) void norm_backward_kernel(
     NormArgs a) {
   constexpr int kTeams = kBlock<TEAM> / TEAM;
   __shared__ float smem[TEAM > kWave ? 2 * 2 * TEAM / kWave : 1];
-  const int lane = threadIdx.x % TEAM;
-  const int64_t teams = a.rows / a.group_rows * a.teams_per_group;
-  const int64_t team = (int64_t) blockIdx.x * kTeams + threadIdx.x / TEAM;
-  if (team >= teams) return;  // whole waves; a team of several is a workgroup
-  const int64_t group = team / a.teams_per_group;
-  const int64_t part = team % a.teams_per_group;
-  const int64_t share =
-      (a.group_rows + a.teams_per_group - 1) / a.teams_per_group;
-  const int64_t first = group * a.group_rows + part * share;
-  int64_t last = first + share;
-  if (last > (group + 1) * a.group_rows) last = (group + 1) * a.group_rows;
+  const int lane = threadIdx.x % TEAM, team = threadIdx.x / TEAM;
+  const int64_t group = blockIdx.x / a.group_blocks;
+  const int64_t part = blockIdx.x % a.group_blocks;
+  const int64_t first = group * a.group_rows + a.group_rows * part / a.group_blocks;
+  const int64_t last = group * a.group_rows + a.group_rows * (part + 1) / a.group_blocks;
   const float inv_dim = 1.f / (float) a.dim;
   int parity = 0;
 
@@ -194,7 +189,7 @@ __global__ __launch_bounds__(kBlock<TEAM>) void norm_backward_kernel(
     }
   }
 
-  for (int64_t row = first; row < last; ++row) {
+  for (int64_t row = first + team; row < last; row += kTeams) {
     const X* x = static_cast<const X*>(a.x) + row * a.dim;
     const Y* dy = static_cast<const Y*>(a.dy) + row * a.dim;
     const X* dr = static_cast<const X*>(a.dr) + row * a.dim;
@@ -297,13 +292,37 @@ __global__ __launch_bounds__(kBlock<TEAM>) void norm_backward_kernel(
     }
   }
 
-  float* out = a.partial + team * a.dim;
-  const int64_t sum_size = teams * a.dim;
-  auto put = [&](const float (&sums)[VPT][8]) {
+  // the workgroup's sums: its teams' in order
+  float* out = a.partial + (int64_t) blockIdx.x * a.dim;
+  const int64_t sum_size = (int64_t) gridDim.x * a.dim;
+  auto put = [&](float (&sums)[VPT][8]) {
+    if constexpr (kTeams > 1) {
+      __shared__ float joined[kTeams > 1 ? (kTeams - 1) * VPT * 8 * TEAM : 1];
+      __syncthreads();
+      if (team) {
 #pragma unroll
-    for (int v = 0; v < VPT; ++v) {
-      const int at = (v * TEAM + lane) * 8;
-      store8(out + at, sums[v], a.dim - at);
+        for (int v = 0; v < VPT; ++v)
+#pragma unroll
+          for (int j = 0; j < 8; ++j)
+            joined[(((team - 1) * VPT + v) * 8 + j) * TEAM + lane] = sums[v][j];
+      }
+      __syncthreads();
+      if (team == 0) {
+#pragma unroll
+        for (int t = 0; t < kTeams - 1; ++t)
+#pragma unroll
+          for (int v = 0; v < VPT; ++v)
+#pragma unroll
+            for (int j = 0; j < 8; ++j)
+              sums[v][j] += joined[((t * VPT + v) * 8 + j) * TEAM + lane];
+      }
+    }
+    if (team == 0) {
+#pragma unroll
+      for (int v = 0; v < VPT; ++v) {
+        const int at = (v * TEAM + lane) * 8;
+        store8(out + at, sums[v], a.dim - at);
+      }
     }
     out += sum_size;
   };
@@ -320,8 +339,8 @@ __global__ __launch_bounds__(kBlock<TEAM>) void norm_backward_kernel(
   }
 }
 
-// Adds the teams' partial rows: dweight and dpost over all teams, dgate over
-// the teams of its group.  blockIdx.x counts the output rows in that order.
+// Adds the partial rows: dweight and dpost over all workgroups, dgate over
+// those of its group.  blockIdx.x counts the output rows in that order.
 constexpr int kSumColumns = 32, kSumRows = 32;
 
 __global__ __launch_bounds__(kSumColumns* kSumRows) void norm_sum_kernel(
@@ -329,28 +348,28 @@ __global__ __launch_bounds__(kSumColumns* kSumRows) void norm_sum_kernel(
   __shared__ float smem[kSumRows][kSumColumns + 1];
   const int column = threadIdx.x % kSumColumns, line = threadIdx.x / kSumColumns;
   const int at = blockIdx.y * kSumColumns + column;
-  const int64_t teams = a.rows / a.group_rows * a.teams_per_group;
+  const int64_t rows = a.rows / a.group_rows * a.group_blocks;
   const float* in = a.partial;
-  int64_t which = blockIdx.x, first = 0, count = teams;
+  int64_t which = blockIdx.x, first = 0, count = rows;
   void* out = nullptr;
   int type = kFloat32;
   if (a.dweight && which-- == 0) {
     out = a.dweight;
     type = a.weight_type;
   }
-  if (!out && a.dweight) in += teams * a.dim;
+  if (!out && a.dweight) in += rows * a.dim;
   if (!out && a.dpost && which-- == 0) {
     out = a.dpost;
     type = a.post_type;
   }
-  if (!out && a.dpost) in += teams * a.dim;
+  if (!out && a.dpost) in += rows * a.dim;
   int64_t row = 0;
   if (!out) {  // `which` is the gate's row now
     out = a.dgate;
     type = a.gate_type;
     row = which;
-    first = which * a.teams_per_group;
-    count = a.teams_per_group;
+    first = which * a.group_blocks;
+    count = a.group_blocks;
   }
   float s = 0.f;
   if (at < a.dim)
@@ -422,9 +441,7 @@ struct Backward {
   const NormArgs& a;
   template <typename X, typename B, typename Y, int TEAM, int VPT>
   int operator()() const {
-    constexpr int kTeams = kBlock<TEAM> / TEAM;
-    const int64_t teams = a.rows / a.group_rows * a.teams_per_group;
-    const int64_t blocks = (teams + kTeams - 1) / kTeams;
+    const int64_t blocks = a.rows / a.group_rows * a.group_blocks;
     const dim3 grid((unsigned) blocks), block(kBlock<TEAM>);
     const hipStream_t stream = static_cast<hipStream_t>(a.stream);
     if (a.post || a.gate)
@@ -458,8 +475,8 @@ int sofa_norm_forward(const sofa_model::NormArgs* a) {
 
 int sofa_norm_backward(const sofa_model::NormArgs* a) {
   using namespace sofa_model;
-  if (!sound(a) || !a->dx || !(a->dr || a->dy) || a->teams_per_group < 1 ||
-      a->teams_per_group > a->group_rows)
+  if (!sound(a) || !a->dx || !(a->dr || a->dy) || a->group_blocks < 1 ||
+      a->rows / a->group_rows > INT32_MAX / a->group_blocks)
     return kBadArgument;
   if ((a->dweight || a->dpost || a->dgate) && !a->partial) return kBadArgument;
   if ((a->dpost && !a->post) || (a->dgate && !a->gate)) return kBadArgument;

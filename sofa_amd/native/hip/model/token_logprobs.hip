@@ -79,9 +79,10 @@ __device__ __forceinline__ Sums wave_join(Sums x) {
   return x;
 }
 
-// Takes 8 more logits; absent ones are -inf.  A NaN or +inf makes s NaN, and
-// with it every result of the row, as the definition has it.
-__device__ __forceinline__ void take(Sums& t, const float (&x)[8]) {
+// Takes 8 more logits and returns the largest; absent ones are -inf.  A NaN or
+// +inf makes s NaN, and with it every result of the row, as the definition has
+// it.
+__device__ __forceinline__ float take(Sums& t, const float (&x)[8]) {
   float most = x[0];
 #pragma unroll
   for (int j = 1; j < 8; ++j) most = fmaxf(most, x[j]);
@@ -100,6 +101,7 @@ __device__ __forceinline__ void take(Sums& t, const float (&x)[8]) {
     t.s += e;
     t.a += e * fmaxf(d, -1e30f);
   }
+  return most;
 }
 
 // ------------------------------------------------------------ alternatives
@@ -125,29 +127,6 @@ __device__ __forceinline__ uint64_t candidate(float x, int token) {
   return (uint64_t) ordered(x) << 32 | (uint32_t) ~token;
 }
 
-__device__ __forceinline__ uint64_t wave_max(uint64_t x) {
-#pragma unroll
-  for (int o = kWave / 2; o > 0; o >>= 1) {
-    const uint64_t y = __shfl_xor((unsigned long long) x, o);
-    x = y > x ? y : x;
-  }
-  return x;
-}
-
-// Each wave collects candidates that beat the last of its best `top` so far,
-// and when its list is full, keeps the best `top` of it.  In random order few
-// pass after the first steps; in the worst (ascending) order every step fills
-// the list, which costs time but no result.
-constexpr int kListSize = 1024;
-constexpr int kPerLane = kListSize / kWave;
-
-struct Best {
-  uint64_t* list;  // kListSize in LDS, this wave's
-  int count;       // the same in every lane
-  uint64_t least;  // what a candidate has to beat
-  int top;
-};
-
 // Orders this wave's accesses to LDS between its lanes.
 __device__ __forceinline__ void wave_sync() {
   __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
@@ -155,54 +134,124 @@ __device__ __forceinline__ void wave_sync() {
   __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
 }
 
-// The best `top` of the list, in falling order, to the list's front.
+// Each wave collects the candidates that reach a threshold: at first the
+// `top`-th best of what its lanes have each seen best in their first loads,
+// which at least `top` logits reach and, in random order, about one in a
+// hundred.  A list of more than 128 is cut to its best `top`, and the last of
+// those is the threshold from then on: a row of 128256 takes one or two such
+// cuts.  In the worst (rising) order every step fills the list, which costs
+// time but no result.
+constexpr int kListSize = 1024;
+constexpr int kPerLane = kListSize / kWave;
+
+struct Best {
+  uint64_t* list;  // kListSize in LDS, this wave's
+  int count;       // the same in every lane
+  uint64_t least;  // the threshold
+  float floor;     // and its logit, below which nothing has to be looked at
+  int top;
+
+  __device__ __forceinline__ void raise(uint64_t to) {
+    if (to <= least) return;
+    least = to;
+    floor = unordered((uint32_t) (to >> 32));
+  }
+};
+
+__device__ __forceinline__ uint64_t read_lane(uint64_t x, int lane) {
+  return (uint64_t) __builtin_amdgcn_readlane((uint32_t) (x >> 32), lane) << 32 |
+         (uint32_t) __builtin_amdgcn_readlane((uint32_t) x, lane);
+}
+
+// Raises the threshold to the `top`-th best of the lanes' best, 0 where a lane
+// has none: as many candidates reach that.  All differ, so their ranks do.
+__device__ __forceinline__ void raise_by_lanes(Best& b, uint64_t most) {
+  int rank = 0;
+#pragma unroll
+  for (int i = 0; i < kWave; ++i) rank += read_lane(most, i) > most;
+  const uint64_t who = __ballot(rank == b.top - 1 && most);
+  if (who) b.raise(read_lane(most, __ffsll((unsigned long long) who) - 1));
+}
+
+// Appends the lanes' candidates that pass.
+__device__ __forceinline__ void append(Best& b, uint64_t c, bool passes) {
+  const uint64_t below = (1ull << threadIdx.x % kWave) - 1;
+  const uint64_t who = __ballot(passes);
+  if (passes) b.list[b.count + __popcll(who & below)] = c;
+  b.count += __popcll(who);
+}
+
+// Cuts a list to its best `top`, in falling order, with zeros where there are
+// fewer.
 __device__ __forceinline__ void keep_best(Best& b) {
   const int lane = threadIdx.x % kWave;
-  uint64_t mine[kPerLane];
   wave_sync();
+  // A long one first loses what is below the `top`-th best of 64 parts of it:
+  // with `top` at most 32 of 64 parts, at least half.
+  while (b.count > 2 * kWave) {
+    uint64_t mine[kPerLane], most = 0;
 #pragma unroll
-  for (int k = 0; k < kPerLane; ++k) {
+    for (int k = 0; k < kPerLane; ++k) {
+      const int at = k * kWave + lane;
+      mine[k] = at < b.count ? b.list[at] : 0;
+      most = mine[k] > most ? mine[k] : most;
+    }
+    raise_by_lanes(b, most);
+    wave_sync();
+    b.count = 0;
+#pragma unroll
+    for (int k = 0; k < kPerLane; ++k)
+      append(b, mine[k], mine[k] && mine[k] >= b.least);
+    wave_sync();
+  }
+  // the place of a candidate is the number of those above it
+  uint64_t mine[2];
+  int rank[2] = {};
+#pragma unroll
+  for (int k = 0; k < 2; ++k) {
     const int at = k * kWave + lane;
     mine[k] = at < b.count ? b.list[at] : 0;
   }
-  uint64_t last = ~0ull, next = 0;
-  for (int i = 0; i < b.top; ++i) {
-    uint64_t most = 0;
+#pragma unroll 8
+  for (int i = 0; i < b.count; ++i) {
+    const uint64_t other = b.list[i];
 #pragma unroll
-    for (int k = 0; k < kPerLane; ++k)
-      most = mine[k] < last && mine[k] > most ? mine[k] : most;
-    most = wave_max(most);
-    last = most;
-    if (lane == i) next = most;
+    for (int k = 0; k < 2; ++k) rank[k] += other > mine[k];
   }
   wave_sync();
-  if (lane < b.top) b.list[lane] = next;
+  if (lane >= b.count && lane < b.top) b.list[lane] = 0;
+#pragma unroll
+  for (int k = 0; k < 2; ++k)
+    if (k * kWave + lane < b.count && rank[k] < b.top) b.list[rank[k]] = mine[k];
   wave_sync();
   if (b.count > b.top) b.count = b.top;
-  b.least = b.count < b.top ? 0 : last;
+  if (b.count == b.top) b.raise(b.list[b.top - 1]);
 }
 
-__device__ __forceinline__ void offer(Best& b, const float (&x)[8], int first,
-                                      int n) {
-  const int lane = threadIdx.x % kWave;
-  const uint64_t below = (1ull << lane) - 1;
-  uint32_t most = 0;
-  const uint32_t least = (uint32_t) (b.least >> 32);
+// `most`: the largest of them; `all`: one of the row may be NaN, which is above
+// every threshold but not found by comparing
+__device__ __forceinline__ void offer(Best& b, const float (&x)[8], float most,
+                                      bool all, int first, int n) {
+  if (!__ballot(n > 0 && (most >= b.floor || all))) return;
 #pragma unroll
   for (int j = 0; j < 8; ++j) {
-    const uint32_t u = j < n ? ordered(x[j]) : 0;
-    most = u > most ? u : most;
-  }
-  if (!__ballot(most >= least && n > 0)) return;
-#pragma unroll
-  for (int j = 0; j < 8; ++j) {
+    const bool may = j < n && (x[j] >= b.floor || all);
+    if (!__ballot(may)) continue;
     const uint64_t c = candidate(x[j], first + j);
-    const bool passes = j < n && c > b.least;
-    const uint64_t who = __ballot(passes);
-    if (passes) b.list[b.count + __popcll(who & below)] = c;
-    b.count += __popcll(who);
+    append(b, c, may && c >= b.least);
   }
-  if (b.count > kListSize - 8 * kWave) keep_best(b);
+  if (b.count > 2 * kWave) keep_best(b);
+}
+
+// The best candidate of 8 logits of which n are there, or `most`
+__device__ __forceinline__ uint64_t better(uint64_t most, const float (&x)[8],
+                                           int first, int n) {
+#pragma unroll
+  for (int j = 0; j < 8; ++j) {
+    const uint64_t c = j < n ? candidate(x[j], first + j) : 0;
+    most = c > most ? c : most;
+  }
+  return most;
 }
 
 template <typename T>
@@ -254,7 +303,7 @@ __global__ __launch_bounds__(kThreads) void logprob_kernel(LogprobArgs a) {
   const int end = min(a.vocab, begin + a.part_size);
 
   Sums t{-INFINITY, 0.f, 0.f};
-  Best best{lists + (TOP ? wave * kListSize : 0), 0, 0, a.top};
+  Best best{lists + (TOP ? wave * kListSize : 0), 0, 0, -INFINITY, a.top};
   constexpr int kLoads = 4;  // vectors in flight a thread
   constexpr int kStep = kThreads * 8;
   int at = begin;
@@ -263,18 +312,31 @@ __global__ __launch_bounds__(kThreads) void logprob_kernel(LogprobArgs a) {
 #pragma unroll
     for (int k = 0; k < kLoads; ++k)
       load8(x + at + k * kStep + threadIdx.x * 8, v[k]);
+    if constexpr (TOP) {
+      if (at == begin) {
+        uint64_t most = 0;
+#pragma unroll
+        for (int k = 0; k < kLoads; ++k)
+          most = better(most, v[k], at + k * kStep + threadIdx.x * 8, 8);
+        raise_by_lanes(best, most);
+      }
+    }
 #pragma unroll
     for (int k = 0; k < kLoads; ++k) {
-      take(t, v[k]);
-      if constexpr (TOP) offer(best, v[k], at + k * kStep + threadIdx.x * 8, 8);
+      const float most = take(t, v[k]);
+      if constexpr (TOP)
+        offer(best, v[k], most, t.s != t.s, at + k * kStep + threadIdx.x * 8, 8);
     }
   }
   for (; at < end; at += kStep) {
     const int first = at + threadIdx.x * 8;
     float v[8];
     load8(x + first, v, end - first, -INFINITY);
-    take(t, v);
-    if constexpr (TOP) offer(best, v, first, end - first);
+    const float most = take(t, v);
+    if constexpr (TOP) {
+      if (at == begin) raise_by_lanes(best, better(0, v, first, end - first));
+      offer(best, v, most, t.s != t.s, first, end - first);
+    }
   }
 
   t = wave_join(t);
@@ -283,10 +345,7 @@ __global__ __launch_bounds__(kThreads) void logprob_kernel(LogprobArgs a) {
     sums[wave][1] = t.s;
     sums[wave][2] = t.a;
   }
-  if constexpr (TOP) {
-    keep_best(best);
-    if (lane >= best.count && lane < a.top) best.list[lane] = 0;
-  }
+  if constexpr (TOP) keep_best(best);
   __syncthreads();
   if (wave) return;
   t = Sums{sums[0][0], sums[0][1], sums[0][2]};
@@ -313,11 +372,10 @@ __global__ __launch_bounds__(kThreads) void logprob_kernel(LogprobArgs a) {
       mine[k] = i < all ? lists[i / a.top * kListSize + i % a.top] : 0;
     }
     wave_sync();
+    Best joined{lists, 0, 0, -INFINITY, a.top};
 #pragma unroll
     for (int k = 0; k < kWaves * kMaxTop / kWave; ++k)
-      lists[k * kWave + lane] = mine[k];
-    wave_sync();
-    Best joined{lists, kWaves * kMaxTop, 0, a.top};
+      append(joined, mine[k], mine[k] != 0);
     keep_best(joined);
     if (lane < a.top) {
       if (a.parts == 1)
@@ -342,19 +400,15 @@ __global__ __launch_bounds__(kWave) void logprob_join_kernel(LogprobArgs a) {
   t = wave_join(t);
   if (lane == 0) finish<T>(a, row, t);
   if constexpr (TOP) {
-    Best best{list, 0, 0, a.top};
+    Best best{list, 0, 0, -INFINITY, a.top};
     const uint64_t* in = a.part_top + row * a.parts * a.top;
     const int all = a.parts * a.top;
     for (int at = 0; at < all; at += kWave) {
       const int i = at + lane;
       const uint64_t c = i < all ? in[i] : 0;
-      const bool passes = c > best.least;
-      const uint64_t who = __ballot(passes);
-      if (passes) list[best.count + __popcll(who & ((1ull << lane) - 1))] = c;
-      best.count += __popcll(who);
+      append(best, c, c && c >= best.least);
       if (best.count > kListSize - kWave) keep_best(best);
     }
-    wave_sync();
     keep_best(best);
     if (lane < a.top) put_top(a, row, lane, list[lane], t);
   }

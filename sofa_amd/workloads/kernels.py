@@ -280,10 +280,11 @@ def _same_split(inner: int, rows: int, t: torch.Tensor, axes: int):
 
 
 def _logprob_split(rows: int, vocab: int) -> Tuple[int, int]:
-    """(parts, part_size): a row goes to one workgroup while there are rows for
-    every compute unit twice over; below that it is cut into parts."""
+    """(parts, part_size): a row goes to one workgroup where there are rows for
+    every compute unit, which then read all that memory gives; below that it is
+    cut into parts."""
     step = 2048  # what a workgroup of 256 threads reads at a time
-    parts = max(1, min(64, -(-512 // rows), -(-vocab // step)))
+    parts = max(1, min(64, -(-256 // rows), -(-vocab // step)))
     size = -(-vocab // (parts * step)) * step
     return -(-vocab // size), size
 
@@ -399,7 +400,7 @@ def token_logprobs(
 
 
 # ------------------------------------------------------------------ residual norm
-def _norm_pack(pointers, x, branch_dtype, y_dtype, weight, post, gate, scale, eps, teams=0):
+def _norm_pack(pointers, x, branch_dtype, y_dtype, weight, post, gate, scale, eps, blocks=0):
     dim = x.shape[-1]
     rows = x.numel() // dim
     group_rows = rows if gate is None else rows * dim // gate.numel()
@@ -407,13 +408,14 @@ def _norm_pack(pointers, x, branch_dtype, y_dtype, weight, post, gate, scale, ep
     return _NORM.pack(
         *pointers, _stream(device), rows, group_rows, eps, scale, dim,
         _TYPES[x.dtype], _TYPES[branch_dtype], _TYPES[y_dtype], _TYPES[weight.dtype],
-        0 if post is None else _TYPES[post.dtype], 0 if gate is None else _TYPES[gate.dtype], teams, device)
+        0 if post is None else _TYPES[post.dtype], 0 if gate is None else _TYPES[gate.dtype], blocks, device)
 
 
-def _norm_teams(rows: int, groups: int, dim: int) -> int:
-    """Teams of the backward pass that share the rows of one gate.  About 512
-    workgroups fill the card twice; more would only add partial sums."""
-    return max(1, min((2048 if dim <= 1024 else 512) // groups, rows // groups))
+def _norm_blocks(rows: int, groups: int, dim: int) -> int:
+    """Workgroups of the backward pass that share the rows of one gate. About 512
+    fill the card twice; more would only add partial sums."""
+    rows //= groups
+    return max(1, min(512 // groups, -(-rows // 4) if dim <= 1024 else rows))
 
 
 def _norm_forward(x, branch, weight, post, gate, scale, eps, out_dtype):
@@ -457,14 +459,14 @@ class _ResidualNorm(torch.autograd.Function):
         dgate = torch.empty_like(gate) if need_gate else None
         dim = x.shape[-1]
         groups = 1 if gate is None else gate.numel() // dim
-        teams = _norm_teams(x.numel() // dim, groups, dim)
+        blocks = _norm_blocks(x.numel() // dim, groups, dim)
         sums = need_weight + need_post + need_gate
-        partial = x.new_empty((sums, groups * teams, dim), dtype=torch.float32) if sums else None
+        partial = x.new_empty((sums, groups * blocks, dim), dtype=torch.float32) if sums else None
         _call("sofa_norm_backward", _norm_pack(
             (x.data_ptr(), _ptr(branch), weight.data_ptr(), _ptr(post), _ptr(gate), 0, 0,
              _ptr(dr), _ptr(dy), dx.data_ptr(), _ptr(dbranch), _ptr(partial),
              _ptr(dweight), _ptr(dpost), _ptr(dgate)),
-            x, branch_dtype or out_dtype, out_dtype, weight, post, gate, scale, eps, teams))
+            x, branch_dtype or out_dtype, out_dtype, weight, post, gate, scale, eps, blocks))
         return dx, dbranch, dweight, dpost, dgate, None, None, None
 
 
