@@ -175,50 +175,80 @@ __device__ __forceinline__ void load_row(bf16x8 (&x)[DP / 16], const bf16* row,
   }
 }
 
-// The transposed result of a wave: the lane's row, in DP / 32 blocks of D;
-// zeros in a row that is not valid, whatever was computed for it.  `low`, if
-// there is one, takes what the rounding took off.
+// Orders this wave's accesses to LDS between its lanes.
+__device__ __forceinline__ void wave_sync() {
+  __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+  __builtin_amdgcn_wave_barrier();
+  __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+}
+
+// The 32 rows of a wave's result, which are its lanes' columns of D, to memory
+// by way of LDS (`stage`: the wave's 32 DP elements), so that whole rows are
+// written: a lane's own pieces are 8 bytes in a row of its own.  Rows that are
+// not valid are zeros, whatever was computed for them; `rows` exist.  `rest`:
+// what rounding took off in place of the result.
 template <int DP>
-__device__ __forceinline__ void store_row(bf16* row,
-                                          const floatx16 (&acc)[DP / 32],
-                                          float factor, bool valid, int dim,
-                                          bf16* low = nullptr) {
-  const int h = threadIdx.x % kWave / 32;
+__device__ __forceinline__ void store_rows(bf16* stage, bf16* to,
+                                           int64_t stride, int rows, int dim,
+                                           const floatx16 (&acc)[DP / 32],
+                                           float factor, bool valid,
+                                           bool rest = false) {
+  constexpr int kChunks = DP / 8;
+  const int lane = threadIdx.x % kWave, h = lane / 32;
+  wave_sync();
 #pragma unroll
   for (int b = 0; b < DP / 32; ++b)
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      const int at = b * 32 + i * 8 + h * 4;
-      bf16x4 x, rest;
+      bf16x4 x;
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
         const float y = valid ? acc[b][i * 4 + j] * factor : 0.f;
         x[j] = (bf16) y;
-        rest[j] = (bf16) (y - (float) x[j]);
+        if (rest) x[j] = (bf16) (y - (float) x[j]);
       }
-      if (at < dim) {
-        *reinterpret_cast<bf16x4*>(row + at) = x;
-        if (low) *reinterpret_cast<bf16x4*>(low + at) = rest;
-      }
+      *reinterpret_cast<bf16x4*>(stage + lds_at<DP>(lane % 32, b * 4 + i) +
+                                 h * 4) = x;
     }
+  wave_sync();
+#pragma unroll
+  for (int p = 0; p < 32 * kChunks / kWave; ++p) {
+    const int row = (p * kWave + lane) / kChunks, chunk = lane % kChunks;
+    if (row < rows && chunk * 8 < dim)
+      *reinterpret_cast<bf16x8*>(to + row * stride + chunk * 8) =
+          *reinterpret_cast<const bf16x8*>(stage + lds_at<DP>(row, chunk));
+  }
 }
 
-// The same in 32 bits
+// The same in 32 bits, 32 columns at a time, rows `dim` apart
 template <int DP>
-__device__ __forceinline__ void store_row(float* row,
-                                          const floatx16 (&acc)[DP / 32],
-                                          bool valid, int dim) {
-  const int h = threadIdx.x % kWave / 32;
+__device__ __forceinline__ void store_rows(bf16* stage, float* to, int rows,
+                                           int dim,
+                                           const floatx16 (&acc)[DP / 32],
+                                           bool valid) {
+  float* buffer = reinterpret_cast<float*>(stage);
+  const int lane = threadIdx.x % kWave, h = lane / 32;
 #pragma unroll
-  for (int b = 0; b < DP / 32; ++b)
+  for (int b = 0; b < DP / 32; ++b) {
+    wave_sync();
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      const int at = b * 32 + i * 8 + h * 4;
       floatx4 x;
 #pragma unroll
       for (int j = 0; j < 4; ++j) x[j] = valid ? acc[b][i * 4 + j] : 0.f;
-      if (at < dim) *reinterpret_cast<floatx4*>(row + at) = x;
+      *reinterpret_cast<floatx4*>(
+          buffer + lane % 32 * 32 + ((i * 2 + h) ^ (lane & 7)) * 4) = x;
     }
+    wave_sync();
+#pragma unroll
+    for (int p = 0; p < 4; ++p) {
+      const int row = p * 8 + lane / 8, at = b * 32 + lane % 8 * 4;
+      if (row < rows && at < dim)
+        *reinterpret_cast<floatx4*>(to + row * dim + at) =
+            *reinterpret_cast<const floatx4*>(
+                buffer + row * 32 + (lane % 8 ^ (row & 7)) * 4);
+    }
+  }
 }
 
 __device__ __forceinline__ float other_half(float x) {
@@ -339,16 +369,20 @@ __global__ __launch_bounds__(kThreads, 2) void attention_forward_kernel(
       tile.template operator()<true>(first, buffer);
   }
 
-  if (row >= a.tokens) return;
   l += other_half(l);
   const bool valid = row < n;
-  const int64_t o_at = batch * a.o_stride[0] + head * a.o_stride[1] +
-                       (int64_t) row * a.o_stride[2];
-  store_row<DP>(a.o + o_at, acc, 1.f / l, valid, a.dim,
-                a.o_low ? a.o_low + o_at : nullptr);
-  if (a.lse && h == 0)
+  if (row < a.tokens && a.lse && h == 0)
     a.lse[(int64_t) bh * a.tokens + row] =
         valid ? m + log2_fast(l) : INFINITY;
+  __syncthreads();  // the tiles are not read any more
+  bf16* stage = k_tiles[0] + wave * 32 * DP;
+  const int64_t o_at = batch * a.o_stride[0] + head * a.o_stride[1] +
+                       (int64_t) wave_row * a.o_stride[2];
+  store_rows<DP>(stage, a.o + o_at, a.o_stride[2], a.tokens - wave_row, a.dim,
+                 acc, 1.f / l, valid);
+  if (a.o_low)
+    store_rows<DP>(stage, a.o_low + o_at, a.o_stride[2], a.tokens - wave_row,
+                   a.dim, acc, 1.f / l, valid, true);
 }
 
 // dQ, and delta for the other kernel
@@ -460,10 +494,12 @@ __global__ __launch_bounds__(kThreads, 2) void attention_dq_kernel(
     else
       tile.template operator()<true>(first, buffer);
   }
-  if (row >= a.tokens) return;
-  store_row<DP>(a.dq + batch * a.dq_stride[0] + head * a.dq_stride[1] +
-                    (int64_t) row * a.dq_stride[2],
-                acc, a.scale, valid, a.dim);
+  __syncthreads();  // the tiles are not read any more
+  store_rows<DP>(k_tiles[0] + wave * 32 * DP,
+                 a.dq + batch * a.dq_stride[0] + head * a.dq_stride[1] +
+                     (int64_t) wave_row * a.dq_stride[2],
+                 a.dq_stride[2], a.tokens - wave_row, a.dim, acc, a.scale,
+                 valid);
 }
 
 // dK and dV, summed over the heads that share them.  A workgroup takes its
@@ -482,8 +518,9 @@ attention_dkv_kernel(AttentionArgs a) {
   constexpr int kLines = kKeepV ? 64 : 32;  // rows of a tile
   constexpr int kBlocks = kLines / 32;
   __shared__ __align__(16) bf16 v_rows[kKeepV ? 8 : kRows * DP];
-  __shared__ __align__(16) bf16 q_tiles[2][kLines * DP];
-  __shared__ __align__(16) bf16 do_tiles[2][kLines * DP];
+  __shared__ __align__(16) bf16 tiles_of[2][2][kLines * DP];
+  bf16(*q_tiles)[kLines * DP] = tiles_of[0];
+  bf16(*do_tiles)[kLines * DP] = tiles_of[1];
   // what the products of a row start from: -lse in units of the scores, and
   // -delta
   __shared__ __align__(16) float lse_tiles[2][kLines];
@@ -633,21 +670,25 @@ attention_dkv_kernel(AttentionArgs a) {
     }
   }
 
-  if (key >= a.tokens) return;
+  __syncthreads();  // the tiles are not read any more
+  bf16* stage = tiles_of[0][0] + wave * 32 * DP;
+  const int rows = a.tokens - wave_key;
   if (a.key_parts > 1) {
     const int64_t size = (int64_t) a.batch * a.kv_heads * a.tokens * a.dim;
     float* out = a.partial + part * 2 * size +
-                 ((int64_t) bh * a.tokens + key) * a.dim;
-    store_row<DP>(out, dk, valid, a.dim);
-    store_row<DP>(out + size, dv, valid, a.dim);
+                 ((int64_t) bh * a.tokens + wave_key) * a.dim;
+    store_rows<DP>(stage, out, rows, a.dim, dk, valid);
+    store_rows<DP>(stage, out + size, rows, a.dim, dv, valid);
     return;
   }
-  store_row<DP>(a.dk + batch * a.dk_stride[0] + kv_head * a.dk_stride[1] +
-                    (int64_t) key * a.dk_stride[2],
-                dk, a.scale, valid, a.dim);
-  store_row<DP>(a.dv + batch * a.dv_stride[0] + kv_head * a.dv_stride[1] +
-                    (int64_t) key * a.dv_stride[2],
-                dv, 1.f, valid, a.dim);
+  store_rows<DP>(stage,
+                 a.dk + batch * a.dk_stride[0] + kv_head * a.dk_stride[1] +
+                     (int64_t) wave_key * a.dk_stride[2],
+                 a.dk_stride[2], rows, a.dim, dk, a.scale, valid);
+  store_rows<DP>(stage,
+                 a.dv + batch * a.dv_stride[0] + kv_head * a.dv_stride[1] +
+                     (int64_t) wave_key * a.dv_stride[2],
+                 a.dv_stride[2], rows, a.dim, dv, 1.f, valid);
 }
 
 // dK and dV as the sum of their parts, in order; 8 elements a thread
