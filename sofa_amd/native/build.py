@@ -10,6 +10,7 @@ from __future__ import annotations
 import os
 import subprocess
 import sys
+import sysconfig
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 BIN = os.path.join(HERE, "bin")
@@ -160,28 +161,51 @@ def build_all(verbose: bool = False) -> None:
 
 
 def _build_model_kernels(hipcc: str, verbose: bool) -> None:
-    """The operators of workloads.kernels: one object per source, compiled side
-    by side (their many variants take a minute each), then linked."""
+    """The operators of workloads.kernels: the kernels, one object per source,
+    compiled side by side (their many variants take a minute each) and linked
+    into libsofamodel, and their binding to torch where torch is installed."""
     src_dir = os.path.join(HERE, "hip", "model")
     dst = os.path.join(LIB, "libsofamodel.so")
-    header = os.path.join(src_dir, "model_ops.h")
+    headers = [os.path.join(src_dir, n) for n in ("model_ops.h", "model_api.h")]
     srcs = [os.path.join(src_dir, n) for n in sorted(os.listdir(src_dir)) if n.endswith(".hip")]
-    if _newer(dst, header, *srcs):
-        return
     objs, running = [], []
-    for src in srcs:
-        obj = os.path.join(LIB, os.path.basename(src)[:-4] + ".o")
-        objs.append(obj)
-        if _newer(obj, header, src):
-            continue
-        cmd = [hipcc] + HIP_FLAGS + ["-std=c++20", "-fPIC", "-c", src, "-o", obj]
+
+    def start(cmd):
         if verbose:
             print("+ " + " ".join(cmd))
         running.append((cmd, subprocess.Popen(cmd)))
+
+    for src in srcs:
+        obj = os.path.join(LIB, os.path.basename(src)[:-4] + ".o")
+        objs.append(obj)
+        if not _newer(obj, src, *headers):
+            start([hipcc] + HIP_FLAGS + ["-std=c++20", "-fPIC", "-c", src, "-o", obj])
+
+    binding = os.path.join(src_dir, "bindings.cc")
+    module, module_obj = os.path.join(LIB, "sofa_model.so"), os.path.join(LIB, "bindings.o")
+    torch_lib = None
+    try:
+        import torch
+        from torch.utils.cpp_extension import include_paths
+
+        torch_lib = os.path.join(os.path.dirname(torch.__file__), "lib")
+    except ImportError:
+        if verbose:
+            print("torch is not installed: the operators of workloads.kernels are not bound")
+    if torch_lib and not _newer(module_obj, binding, headers[1]):
+        include = include_paths() + [f"{ROCM}/include", sysconfig.get_paths()["include"]]
+        start(["g++", "-O2", "-std=c++17", "-fPIC", "-fvisibility=hidden", "-D__HIP_PLATFORM_AMD__", "-DUSE_ROCM",
+               f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}"]
+              + [f"-I{i}" for i in include] + ["-c", binding, "-o", module_obj])
+
     failed = [cmd for cmd, p in running if p.wait() != 0]
     if failed:
         raise subprocess.CalledProcessError(1, failed[0])
-    _run([hipcc, f"--offload-arch={GFX_ARCH}", "-shared", "-o", dst] + objs, verbose)
+    if not _newer(dst, *objs):
+        _run([hipcc, f"--offload-arch={GFX_ARCH}", "-shared", "-o", dst] + objs, verbose)
+    if torch_lib and not _newer(module, module_obj, dst):
+        _run(["g++", "-shared", "-o", module, module_obj, f"-L{torch_lib}", "-ltorch_python", "-ltorch", "-ltorch_cpu",
+              "-lc10_hip", "-lc10", f"-L{LIB}", "-lsofamodel", "-Wl,-rpath,$ORIGIN"], verbose)
 
 
 if __name__ == "__main__":

@@ -33,24 +33,6 @@
 namespace sofa_model {
 namespace {
 
-struct AttentionArgs {
-  const bf16 *q, *k, *v;  // [batch][heads][tokens][dim] by strides, dim dense
-  bf16* o;
-  bf16* o_low;            // what rounding took off o, laid out like it; or null
-  float* lse;             // [batch][heads][tokens], base 2; +inf: no keys
-  const int* lengths;     // [batch] valid tokens, or null
-  const bf16* dout;
-  float* delta;           // [batch][heads][tokens]
-  bf16 *dq, *dk, *dv;
-  float* partial;         // [key_parts][2][batch][kv_heads][tokens][dim], or null
-  void* stream;
-  int64_t q_stride[3], k_stride[3], v_stride[3], o_stride[3];  // batch, head,
-  int64_t dout_stride[3], dq_stride[3], dk_stride[3], dv_stride[3];  // token
-  float scale;
-  int batch, heads, kv_heads, tokens, dim, causal, key_parts, device;
-};
-static_assert(sizeof(AttentionArgs) == 344, "as the caller packs it");
-
 typedef bf16 bf16x4 __attribute__((ext_vector_type(4)));
 typedef bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef short shortx4 __attribute__((ext_vector_type(4)));
@@ -61,9 +43,6 @@ constexpr int kThreads = 256;
 constexpr int kWaves = 4;
 constexpr int kRows = kWaves * 32;  // rows a workgroup owns
 constexpr int kTile = 64;           // rows of the other side at a time
-// between tokens, in elements: kTile rows are within 32-bit offsets
-constexpr int64_t kMaxStride = 1 << 24;
-constexpr int kMaxKeyParts = 8;
 
 // Where the 8 elements `chunk` of `row` of a tile are in LDS.  A row is 256 or
 // 128 bytes and the banks 256, so one chunk of all rows falls on the same banks;
@@ -97,7 +76,7 @@ __device__ __forceinline__ void load_tile(const bf16* tile, int64_t stride,
   const uint32_t row = threadIdx.x / kChunks;
   const int chunk = threadIdx.x % kChunks ^ swizzle<DP>(row);
   const uint32_t at = min(chunk, dim / 8 - 1) * 8;
-  const uint32_t step = (uint32_t) stride;  // up to kMaxStride
+  const uint32_t step = (uint32_t) stride;  // up to kMaxTokenStride
   to += __builtin_amdgcn_readfirstlane(threadIdx.x / kWave) * kWave * 8;
 #pragma unroll
   for (int p = 0; p < ROWS / kStep; ++p) {
@@ -750,12 +729,12 @@ int backward(const AttentionArgs& a) {
 bool sound(const AttentionArgs* a) {
   if (!a || a->batch <= 0 || a->heads <= 0 || a->kv_heads <= 0 ||
       a->heads % a->kv_heads || a->tokens <= 0 || a->dim <= 0 || a->dim % 8 ||
-      a->dim > 128 || !a->q || !a->k || !a->v || !a->o)
+      a->dim > kMaxHeadDim || !a->q || !a->k || !a->v || !a->o)
     return false;
   for (const int64_t* stride : {a->q_stride, a->k_stride, a->v_stride})
-    if (stride[2] < 0 || stride[2] > kMaxStride) return false;
+    if (stride[2] < 0 || stride[2] > kMaxTokenStride) return false;
   // the grid, and row numbers up to the end of a block
-  return a->tokens <= (1 << 24) &&
+  return a->tokens <= kMaxTokens &&
          (int64_t) a->batch * a->heads * ((a->tokens + kRows - 1) / kRows) <=
              INT32_MAX / kMaxKeyParts;
 }
@@ -779,7 +758,7 @@ int sofa_attention_backward(const sofa_model::AttentionArgs* a) {
   using namespace sofa_model;
   if (!sound(a) || !a->dout || !a->o_low || !a->lse || !a->delta || !a->dq || !a->dk ||
       !a->dv || a->key_parts < 1 || a->key_parts > kMaxKeyParts ||
-      (a->key_parts > 1 && !a->partial) || a->dout_stride[2] < 0 || a->dout_stride[2] > kMaxStride)
+      (a->key_parts > 1 && !a->partial) || a->dout_stride[2] < 0 || a->dout_stride[2] > kMaxTokenStride)
     return kBadArgument;
   DeviceGuard guard(a->device);
   if (guard.status()) return guard.status();

@@ -6,18 +6,11 @@
 
 #include <hip/hip_runtime.h>
 
-#include <cstdint>
+#include "model_api.h"
 
 namespace sofa_model {
 
-using bf16 = __bf16;
 using fp16 = _Float16;
-
-// element type codes, as kernels.py numbers them
-enum Type : int { kFloat32 = 0, kBFloat16 = 1, kFloat16 = 2 };
-
-// what a C entry returns: 0, a positive hipError_t, or kBadArgument
-constexpr int kBadArgument = -1;
 
 constexpr int kWave = 64;
 

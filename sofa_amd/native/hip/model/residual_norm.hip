@@ -22,22 +22,6 @@
 namespace sofa_model {
 namespace {
 
-struct NormArgs {
-  const void *x, *branch, *weight, *post, *gate;  // branch, post, gate: or null
-  void *r, *y;                                    // r: null without a branch
-  const void *dr, *dy;                            // either may be null
-  void *dx, *dbranch;                             // dbranch: or null
-  float* partial;  // [sums][workgroups][dim]: dweight, then dpost, then dgate
-  void *dweight, *dpost, *dgate;                  // each or null
-  void* stream;
-  int64_t rows, group_rows;  // rows, and rows that share one gate
-  float eps, scale;
-  int dim, x_type, branch_type, y_type, weight_type, post_type, gate_type;
-  int group_blocks;          // backward: workgroups that share a gate's rows
-  int device;
-};
-static_assert(sizeof(NormArgs) == 192, "as the caller packs it");
-
 // Sums of N <= 2 values over a team, in every thread of it.  `parity` alternates
 // between calls, so that one barrier is enough: a buffer is written again
 // only after the barrier of the call between.
@@ -455,7 +439,7 @@ struct Backward {
 };
 
 bool sound(const NormArgs* a) {
-  return a && a->rows > 0 && a->rows <= INT32_MAX && a->dim > 0 && a->dim <= 16384 &&
+  return a && a->rows > 0 && a->rows <= INT32_MAX && a->dim > 0 && a->dim <= kMaxNormDim &&
          a->group_rows > 0 && a->rows % a->group_rows == 0 && a->x &&
          a->weight && (a->branch || !(a->post || a->gate));
 }

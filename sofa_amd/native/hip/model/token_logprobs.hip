@@ -21,31 +21,6 @@ namespace {
 
 constexpr int kThreads = 256;
 constexpr int kWaves = kThreads / kWave;
-constexpr int kMaxTop = 32;
-constexpr int kMaxParts = 64;
-
-struct LogprobArgs {
-  const void* logits;
-  const int64_t* tokens;
-  float *logprob, *entropy, *lse;
-  int64_t* top_ids;    // [rows][top], or null
-  float* top_logprobs;
-  // when parts > 1: (m, s, a) and the top candidates of each part of a row
-  float* part_sums;    // [rows][parts][3]
-  uint64_t* part_top;  // [rows][parts][top]
-  const float *dlogprob, *dentropy;  // either may be null
-  void* dlogits;                     // [rows][vocab]
-  void* stream;
-  int64_t rows, inner;        // row i is at (i / inner) outer_stride
-  int64_t outer_stride, inner_stride;  //  + (i % inner) inner_stride elements
-  int64_t grad_outer_stride, grad_inner_stride;    // of dlogprob
-  int64_t grad2_outer_stride, grad2_inner_stride;  // of dentropy
-  int64_t token_outer_stride, token_inner_stride;
-  int64_t ignore_index;
-  int vocab, top, parts, part_size;  // part_size: a multiple of kStep
-  int type, device;
-};
-static_assert(sizeof(LogprobArgs) == 216, "as the caller packs it");
 
 __device__ __forceinline__ int64_t place(int64_t row, int64_t inner,
                                          int64_t outer_stride,
@@ -506,9 +481,9 @@ int backward(const LogprobArgs& a) {
 
 bool sound(const LogprobArgs* a) {
   return a && a->logits && a->tokens && a->logprob && a->entropy && a->lse &&
-         a->rows > 0 && a->inner > 0 && a->vocab > 0 && a->vocab <= 1 << 30 &&
+         a->rows > 0 && a->inner > 0 && a->vocab > 0 && a->vocab <= kMaxVocab &&
          a->parts > 0 &&
-         a->parts <= kMaxParts && a->part_size > 0 &&
+         a->parts <= kMaxVocabParts && a->part_size > 0 &&
          (int64_t) a->parts * a->part_size >= a->vocab &&
          (int64_t) (a->parts - 1) * a->part_size < a->vocab &&
          a->rows <= INT32_MAX / a->parts;

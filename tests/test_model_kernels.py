@@ -113,28 +113,43 @@ def test_llama_refuses_unknown_kernels():
         Llama(vocab=16, dim=16, n_layers=1, n_heads=2, n_kv_heads=1, hidden=16, max_seq=8, kernels="fast")
 
 
-def test_argument_structures_are_whole():
-    """What is packed is what the C structures hold (static_assert there)."""
-    assert [s.size for s in (kernels._ATTENTION, kernels._LOGPROBS, kernels._NORM)] == [344, 216, 192]
+@pytest.fixture(scope="module")
+def ops():
+    from sofa_amd.native.build import build_all
+
+    if not os.path.exists(os.path.join(REPO, "sofa_amd", "native", "lib", "sofa_model.so")):
+        build_all()
+    return kernels._ops()
 
 
-def test_rows_in_two_levels():
+def test_rows_in_two_levels(ops):
     t = torch.zeros(4, 6, 8)
-    assert kernels._two_level(t, 2) == (24, 0, 8)
-    assert kernels._two_level(t[:, :-1], 2) == (5, 48, 8)
-    assert kernels._two_level(t[:1, :1], 2)[0] == 1
-    assert kernels._two_level(t[:1, :1, ::2], 2) == (1, 0, 0)
-    assert kernels._two_level(t.transpose(0, 1), 2) == (4, 8, 48)
-    assert kernels._two_level(torch.zeros(()).expand(4, 6), 2) == (24, 0, 0)
-    assert kernels._two_level(torch.zeros(3, 4, 5, 6)[:, :2, :3], 3) is None
+    assert ops.two_level(t, 2) == [24, 0, 8]
+    assert ops.two_level(t[:, :-1], 2) == [5, 48, 8]
+    assert ops.two_level(t[:1, :1], 2) == [1, 0, 0]
+    assert ops.two_level(t.transpose(0, 1), 2) == [4, 8, 48]
+    assert ops.two_level(torch.zeros(()).expand(4, 6), 2) == [24, 0, 0]
+    assert ops.two_level(torch.zeros(3, 4, 5, 6)[:, :2, :3], 3) is None
+    assert ops.two_level(torch.zeros(3, 4, 5, 6)[:, :, :3], 3) == [3, 30, 6]
 
 
-@pytest.mark.parametrize("rows", [1, 2, 7, 255, 511, 512, 513, 8192])
+@pytest.mark.parametrize("rows", [1, 2, 7, 255, 256, 257, 513, 8192])
 @pytest.mark.parametrize("vocab", [1, 9, 2048, 2049, 50001, 128256, 1 << 30])
-def test_parts_cover_a_row(rows, vocab):
-    parts, size = kernels._logprob_split(rows, vocab)
+def test_parts_cover_a_row(ops, rows, vocab):
+    parts, size = ops.vocab_parts(rows, vocab)
     assert 1 <= parts <= 64 and size % 2048 == 0
     assert (parts - 1) * size < vocab <= parts * size
+
+
+@pytest.mark.parametrize("rows, groups, dim", [(1, 1, 64), (3, 3, 2000), (700, 700, 40), (8192, 1, 4096), (8192, 2, 512)])
+def test_norm_blocks(ops, rows, groups, dim):
+    assert 1 <= ops.norm_blocks(rows, groups, dim) <= rows // groups
+
+
+@pytest.mark.parametrize("tokens", [1, 33, 512, 2048, 1 << 20])
+def test_key_parts(ops, tokens):
+    for causal in (True, False):
+        assert 1 <= ops.key_parts(1, 8, 2, tokens, 128, causal) <= 8
 
 
 # ------------------------------------------------------------------ attention
@@ -705,6 +720,25 @@ def _run(q, k, v, do, x, tokens, g, h, res, w):
     grads = torch.autograd.grad((r, y, out.logprob, out.entropy), leaves,
                                 (res.detach(), do.transpose(1, 2).reshape(2, 150, 256), g, h))
     return [t.detach() for t in (o, r, y, *out, *grads)]
+
+
+@pytest.mark.gpu
+def test_first_derivatives_only():
+    """A recorded backward pass gives the same gradients; a second one is refused."""
+    q, k, v, do = attention_case(1, 2, 1, 20, 16)
+    x, tokens, g, _ = logits_case(3, 50, FP32)
+    res, w = torch.randn(3, 40, device="cuda", requires_grad=True), torch.ones(40, device="cuda", requires_grad=True)
+    x.requires_grad_()
+    for out, leaf, grad in (
+        (kernels.attention(q, k, v), q, do),
+        (kernels.token_logprobs(x, tokens).logprob, x, g),
+        (kernels.residual_norm(res, res * 0.5, w)[1], w, torch.randn(3, 40, device="cuda")),
+    ):
+        (plain,) = torch.autograd.grad(out, leaf, grad, retain_graph=True)
+        (first,) = torch.autograd.grad(out, leaf, grad, create_graph=True)
+        assert torch.equal(first, plain) and first.requires_grad
+        with pytest.raises(RuntimeError, match="first derivatives only"):
+            torch.autograd.grad(first.sum(), leaf)
 
 
 @pytest.mark.gpu
