@@ -39,7 +39,9 @@ def _run(cmd, verbose=False):
     subprocess.run(cmd, check=True)
 
 
-def build_all(verbose: bool = False) -> None:
+def build_all(verbose: bool = False, model: bool = True) -> None:
+    """model: the operators of workloads.kernels as well, which recording does
+    not need and which take a minute."""
     os.makedirs(BIN, exist_ok=True)
     os.makedirs(LIB, exist_ok=True)
 
@@ -157,7 +159,8 @@ def build_all(verbose: bool = False) -> None:
             cmd += ["-L" + LIB, "-lsofahip", "-Wl,-rpath,$ORIGIN/../lib"]
         _run(cmd, verbose)
 
-    _build_model_kernels(hipcc, verbose)
+    if model:
+        _build_model_kernels(hipcc, verbose)
 
 
 def _build_model_kernels(hipcc: str, verbose: bool) -> None:

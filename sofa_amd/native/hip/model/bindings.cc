@@ -52,7 +52,10 @@ int type_of(at::ScalarType t) {
                               : sofa_model::kFloat16;
 }
 
-Tensor dense(const Tensor& t) { return t.defined() ? t.contiguous() : t; }
+// The values in memory are a tensor's own unless it is a lazily negated view.
+Tensor dense(const Tensor& t) {
+  return t.defined() ? t.resolve_neg().contiguous() : t;
+}
 
 int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
@@ -247,12 +250,12 @@ std::optional<Split> two_level(const Tensor& t, int64_t axes) {
 // t, or a copy, and its strides over rows that are split at `inner`
 std::tuple<Tensor, int64_t, int64_t> same_split(int64_t inner, int64_t rows,
                                                 const Tensor& t, int64_t axes) {
-  if (const auto s = two_level(t, axes)) {
+  if (const auto s = t.is_neg() ? std::nullopt : two_level(t, axes)) {
     if (s->inner == inner) return {t, s->outer_stride, s->inner_stride};
     if (s->inner >= rows)  // one level: it can be split anywhere
       return {t, inner * s->inner_stride, s->inner_stride};
   }
-  return {t.contiguous(), inner, 1};
+  return {dense(t), inner, 1};
 }
 
 // A row goes to one workgroup where there are rows for every compute unit, which
@@ -269,9 +272,10 @@ std::pair<int, int> vocab_parts(int64_t rows, int64_t vocab) {
 
 // dense rows in two levels
 Tensor logit_rows(const Tensor& logits) {
-  if (logits.stride(-1) == 1 && two_level(logits, logits.dim() - 1))
+  if (!logits.is_neg() && logits.stride(-1) == 1 &&
+      two_level(logits, logits.dim() - 1))
     return logits;
-  return logits.contiguous();
+  return dense(logits);
 }
 
 LogprobArgs logprob_args(const Tensor& logits, Tensor& tokens, int64_t top,

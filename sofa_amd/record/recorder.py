@@ -109,7 +109,7 @@ def ensure_native_built(verbose: bool = False) -> bool:
     try:
         from ..native.build import build_all
 
-        build_all(verbose=verbose)
+        build_all(verbose=verbose, model=False)
     except Exception as e:  # pragma: no cover
         p.print_warning(f"native build failed: {e}")
     return all(os.path.exists(x) for x in needed)

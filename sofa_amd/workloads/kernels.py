@@ -102,7 +102,7 @@ def attention(
         raise ValueError(f"attention: {heads} heads cannot share {k.shape[1]} key heads")
     if dim < 8 or dim % 8 or dim > MAX_HEAD_DIM:
         raise ValueError(f"attention: dim has to be a multiple of 8 up to {MAX_HEAD_DIM}, got {dim}")
-    if tokens > MAX_TOKENS or batch * heads * -(-tokens // 128) > 2**31 - 1:
+    if tokens > MAX_TOKENS or batch * heads * -(-tokens // 128) > 2**28 - 1:
         raise ValueError(f"attention: {tuple(q.shape)} is too large")
     if scale is None:
         scale = 1.0 / math.sqrt(dim)

@@ -462,6 +462,9 @@ def test_token_logprobs_views():
     check_logprobs(x[0, 0], ids[0, 0], 2, g[0, 0], g[0, 1])
     check_logprobs(x.view(b, t, 1, vocab).expand(b, t, 2, vocab)[:, :3], ids.view(b, t, 1).expand(b, t, 2)[:, :3], 1)
     check_logprobs(x[..., 1:], ids % (vocab - 1), 2, torch.ones((), device="cuda").expand(b, t), None)
+    negated = torch.view_as_complex(torch.stack((x[0].float(), x[1].float()), -1)).conj().imag
+    assert negated.is_neg()
+    assert torch.equal(kernels.token_logprobs(negated, ids[0]).logprob, kernels.token_logprobs(-x[1].float(), ids[0]).logprob)
     # a gradient through a mean is expanded
     leaf = x.clone().requires_grad_()
     (got,) = torch.autograd.grad(kernels.token_logprobs(leaf, ids).logprob.mean(), leaf)
