@@ -43,6 +43,7 @@ constexpr int kThreads = 256;
 constexpr int kWaves = 4;
 constexpr int kRows = kWaves * 32;  // rows a workgroup owns
 constexpr int kTile = 64;           // rows of the other side at a time
+constexpr int kShort = 256;         // tokens up to which dS has 16 bits
 
 // Where the 8 elements `chunk` of `row` of a tile are in LDS.  A row is 256 or
 // 128 bytes and the banks 256, so one chunk of all rows falls on the same banks;
@@ -133,6 +134,16 @@ __device__ __forceinline__ bf16x8 rounded(const floatx16& d, int part) {
   bf16x8 r;
 #pragma unroll
   for (int j = 0; j < 8; ++j) r[j] = (bf16) d[part * 8 + j];
+  return r;
+}
+
+// What that rounding took off
+__device__ __forceinline__ bf16x8 rest_of(const floatx16& d, int part,
+                                          bf16x8 rounded) {
+  bf16x8 r;
+#pragma unroll
+  for (int j = 0; j < 8; ++j)
+    r[j] = (bf16) (d[part * 8 + j] - (float) rounded[j]);
   return r;
 }
 
@@ -364,8 +375,13 @@ __global__ __launch_bounds__(kThreads, 2) void attention_forward_kernel(
                    a.dim, acc, 1.f / l, valid, true);
 }
 
-// dQ, and delta for the other kernel
-template <int DP, bool CAUSAL>
+// dQ, and delta for the other kernel.
+//
+// SHORT: dS is taken with 16 bits, as its rounding and what that took off. In
+// long rows its rounding is one of many and leaves dQ and dK 1.4 times as far
+// off as their own rounding does; in short ones it was up to 1.6 times. There
+// the products that this adds are not what takes the time.
+template <int DP, bool CAUSAL, bool SHORT>
 __global__ __launch_bounds__(kThreads, 2) void attention_dq_kernel(
     AttentionArgs a) {
   __shared__ __align__(16) bf16 k_tiles[2][kTile * DP];
@@ -453,8 +469,11 @@ __global__ __launch_bounds__(kThreads, 2) void attention_dq_kernel(
       for (int p = 0; p < 2 * kBlocks; ++p) {
         const bf16x8 ds = rounded(s[p / 2], p % 2);
 #pragma unroll
-        for (int c = 0; c < DP / 32; ++c)
-          acc[c] = mfma(column_operand<DP>(k_tile, line + p * 16, c), ds, acc[c]);
+        for (int c = 0; c < DP / 32; ++c) {
+          const bf16x8 keys = column_operand<DP>(k_tile, line + p * 16, c);
+          acc[c] = mfma(keys, ds, acc[c]);
+          if (SHORT) acc[c] = mfma(keys, rest_of(s[p / 2], p % 2, ds), acc[c]);
+        }
       }
     }
   };
@@ -490,7 +509,7 @@ __global__ __launch_bounds__(kThreads, 2) void attention_dq_kernel(
 // is in LDS then and tiles have 32 rows.  With V in registers too and one
 // workgroup (of 64 rows a tile) the same 2 x 4096 tokens, 32/8 heads, took 1.26
 // ms in place of 1.04, without a mask.
-template <int DP, bool CAUSAL>
+template <int DP, bool CAUSAL, bool SHORT>
 __global__ __launch_bounds__(kThreads, 2) void
 attention_dkv_kernel(AttentionArgs a) {
   constexpr bool kKeepV = DP <= 64;
@@ -620,7 +639,9 @@ attention_dkv_kernel(AttentionArgs a) {
 #pragma unroll
       for (int c = 0; c < DP / 32; ++c) {
         dv[c] = mfma(column_operand<DP>(do_tile, p * 16, c), probs, dv[c]);
-        dk[c] = mfma(column_operand<DP>(q_tile, p * 16, c), ds, dk[c]);
+        const bf16x8 rows = column_operand<DP>(q_tile, p * 16, c);
+        dk[c] = mfma(rows, ds, dk[c]);
+        if (SHORT) dk[c] = mfma(rows, rest_of(dp[p / 2], p % 2, ds), dk[c]);
       }
     }
   };
@@ -704,15 +725,15 @@ int forward(const AttentionArgs& a) {
   return (int) hipGetLastError();
 }
 
-template <int DP, bool CAUSAL>
+template <int DP, bool CAUSAL, bool SHORT>
 int backward(const AttentionArgs& a) {
   const int64_t blocks = (a.tokens + kRows - 1) / kRows;
-  hipLaunchKernelGGL((attention_dq_kernel<DP, CAUSAL>),
+  hipLaunchKernelGGL((attention_dq_kernel<DP, CAUSAL, SHORT>),
                      dim3((unsigned) (blocks * a.batch * a.heads)),
                      dim3(kThreads), 0, static_cast<hipStream_t>(a.stream), a);
   int status = (int) hipGetLastError();
   if (status) return status;
-  hipLaunchKernelGGL((attention_dkv_kernel<DP, CAUSAL>),
+  hipLaunchKernelGGL((attention_dkv_kernel<DP, CAUSAL, SHORT>),
                      dim3((unsigned) (blocks * a.batch * a.kv_heads *
                                       a.key_parts)),
                      dim3(kThreads), 0, static_cast<hipStream_t>(a.stream), a);
@@ -724,6 +745,14 @@ int backward(const AttentionArgs& a) {
                      dim3((unsigned) ((threads + kThreads - 1) / kThreads)),
                      dim3(kThreads), 0, static_cast<hipStream_t>(a.stream), a);
   return (int) hipGetLastError();
+}
+
+template <int DP>
+int backward(const AttentionArgs& a) {
+  const bool is_short = a.tokens <= kShort;
+  if (a.causal)
+    return is_short ? backward<DP, true, true>(a) : backward<DP, true, false>(a);
+  return is_short ? backward<DP, false, true>(a) : backward<DP, false, false>(a);
 }
 
 bool sound(const AttentionArgs* a) {
@@ -762,9 +791,7 @@ int sofa_attention_backward(const sofa_model::AttentionArgs* a) {
     return kBadArgument;
   DeviceGuard guard(a->device);
   if (guard.status()) return guard.status();
-  if (a->dim <= 64)
-    return a->causal ? backward<64, true>(*a) : backward<64, false>(*a);
-  return a->causal ? backward<128, true>(*a) : backward<128, false>(*a);
+  return a->dim <= 64 ? backward<64>(*a) : backward<128>(*a);
 }
 
 }  // extern "C"

@@ -11,9 +11,10 @@ Run directly for a profiled step stress:
     sofa stat "python -m sofa_amd.workloads.llama --layers 8 --steps 3"
 
 `--kernels hip` (`Llama(kernels="hip")`) runs attention, the residual norms and
-the loss as the fused kernels of workloads.kernels in place of ATen: the same
-parameters and mathematics in about a tenth of the kernel launches outside the
-matrix products, for profiling a step as a tuned trainer would run it.
+the loss as the fused kernels of workloads.kernels in place of ATen, for
+profiling a step as a tuned trainer would run it: the same parameters and
+mathematics, 8 layers of 2 x 2048 tokens in 113 ms a step in place of 132, with
+a fifth fewer events to trace.
 """
 
 from __future__ import annotations
