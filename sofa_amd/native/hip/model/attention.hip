@@ -19,14 +19,23 @@
 // are, if that product takes its k in the order
 //   slot (h, j) -> 4 h + j (j < 4), 8 + 4 h + j - 4 (j >= 4)
 // of each 16.  Its A operand is read from LDS with ds_read_b64_tr_b16, which
-// gives a lane 4 rows of one column, in that same order.  P and dS are rounded
-// to bf16 for it: 2^-8 relative at most, as in the results themselves; sums
-// stay in 32 bits.  Only delta, which dP - delta almost cancels in short rows,
-// takes more of o than its 8 bits: the forward pass keeps what the rounding
-// took off as well (with o's own rounding dQ and dK of 32 tokens were 3.1e-3
-// off, 1.9 times what the rounding of the results is).
-// delta, though, is a difference that short rows almost cancel: it is taken
-// of o in 16 bits, kept as o and what its rounding took off.
+// gives a lane 4 rows of one column, in that same order.
+//
+// Roundings: P and dS to bf16 for their products, 2^-8 relative at most, as in
+// the results themselves; sums stay in 32 bits.  Only delta, which dP - delta
+// almost cancels in short rows, takes more of O than its 8 bits: the forward
+// pass keeps what the rounding took off as well (with O's own rounding dQ and
+// dK of 32 tokens were 1.9 times as far off as their own rounding leaves them).
+//
+// Measured at 32 query and 8 key heads of 128, causal, in products' TFLOP/s
+// (2, 3 and 4 products; a large library product reaches 1220):
+//                  2 x 2048      2 x 4096       1 x 8192 tokens
+//   forward        93 us  740    315 us  870    565 us  970
+//   dQ            125 us  825    440 us  935    765 us 1080
+//   dK, dV        150 us  915    580 us  950   1075 us 1020
+// What bounds them is the issue of a wave's own instructions: products take 40 %
+// of its cycles, exponentials and their surroundings as many, and two waves on
+// a SIMD (256 registers each) fill each other's gaps only in part.
 
 #include "model_ops.h"
 
@@ -49,7 +58,8 @@ constexpr int kShort = 256;         // tokens up to which dS has 16 bits
 // 128 bytes and the banks 256, so one chunk of all rows falls on the same banks;
 // the exclusive or moves it such that what one cycle pair reads is on different
 // ones: 16 rows of one chunk (a row operand), and 4 rows by 4 chunks (a column
-// operand).  Its lower two bits tell rows 4 apart, the next those 1 apart.
+// operand).  Its lower two bits tell rows 4 apart, the next those 1 apart.  (With
+// pairs of chunks moved by 8 rows, 40 % of LDS cycles were conflicts.)
 template <int DP>
 __device__ __forceinline__ int swizzle(int row) {
   return DP == 128 ? (row & 3) << 2 | (row >> 2 & 3)
@@ -92,8 +102,9 @@ __device__ __forceinline__ void load_tile(const bf16* tile, int64_t stride,
 }
 
 // All of the workgroup's tiles on their way are there.  Reads of LDS wait for
-// this wave's own loads before that: the next ones start where no more reads
-// follow for some time, after the scores' products.
+// this wave's own loads before that, so the next ones start where no more reads
+// follow for some time, after the scores' products.  Staged in registers instead,
+// for a whole tile's time, the forward pass took 8 % more.
 __device__ __forceinline__ void arrived() {
   __builtin_amdgcn_s_waitcnt(0x0f70);  // vmcnt(0)
   __syncthreads();
@@ -439,7 +450,8 @@ __global__ __launch_bounds__(kThreads, 2) void attention_dq_kernel(
     load_tile<DP>(v + first * a.v_stride[2], a.v_stride[2], n - first, a.dim,
                   v_tiles[buffer]);
   };
-  // 32 BLOCKS keys at a time
+  // 32 kBlocks keys at a time: short heads gain more from a third workgroup on
+  // the compute unit (168 registers) than from two independent chains
   constexpr int kBlocks = DP <= 64 ? 1 : 2;
   auto tile = [&]<bool MASKED>(int first, int buffer) {
     const bf16 *k_tile = k_tiles[buffer], *v_tile = v_tiles[buffer];
@@ -573,12 +585,13 @@ attention_dkv_kernel(AttentionArgs a) {
     if (step >= stop) return;
     const int head = kv_head * group + step / tiles;
     const int first = start + (tiles - 1 - step % tiles) * kLines;
-    load_tile<DP, kLines>(a.q + batch * a.q_stride[0] + head * a.q_stride[1] +
-                      first * a.q_stride[2],
-                  a.q_stride[2], n - first, a.dim, q_tiles[buffer]);
-    load_tile<DP, kLines>(a.dout + batch * a.dout_stride[0] + head * a.dout_stride[1] +
-                      first * a.dout_stride[2],
-                  a.dout_stride[2], n - first, a.dim, do_tiles[buffer]);
+    load_tile<DP, kLines>(a.q + batch * a.q_stride[0] +
+                              head * a.q_stride[1] + first * a.q_stride[2],
+                          a.q_stride[2], n - first, a.dim, q_tiles[buffer]);
+    load_tile<DP, kLines>(
+        a.dout + batch * a.dout_stride[0] + head * a.dout_stride[1] +
+            first * a.dout_stride[2],
+        a.dout_stride[2], n - first, a.dim, do_tiles[buffer]);
     // +inf makes every probability of a row that is not there 0
     lse = INFINITY;
     delta = 0.f;
@@ -762,10 +775,10 @@ bool sound(const AttentionArgs* a) {
     return false;
   for (const int64_t* stride : {a->q_stride, a->k_stride, a->v_stride})
     if (stride[2] < 0 || stride[2] > kMaxTokenStride) return false;
-  // the grid, and row numbers up to the end of a block
+  // row numbers up to the end of a block, and a launch's 2^32 threads
   return a->tokens <= kMaxTokens &&
          (int64_t) a->batch * a->heads * ((a->tokens + kRows - 1) / kRows) <=
-             INT32_MAX / kMaxKeyParts;
+             kMaxBlocks;
 }
 
 }  // namespace
@@ -787,7 +800,10 @@ int sofa_attention_backward(const sofa_model::AttentionArgs* a) {
   using namespace sofa_model;
   if (!sound(a) || !a->dout || !a->o_low || !a->lse || !a->delta || !a->dq || !a->dk ||
       !a->dv || a->key_parts < 1 || a->key_parts > kMaxKeyParts ||
-      (a->key_parts > 1 && !a->partial) || a->dout_stride[2] < 0 || a->dout_stride[2] > kMaxTokenStride)
+      (a->key_parts > 1 && !a->partial) || a->dout_stride[2] < 0 ||
+      a->dout_stride[2] > kMaxTokenStride ||
+      (int64_t) a->batch * a->kv_heads * a->key_parts *
+              ((a->tokens + kRows - 1) / kRows) > kMaxBlocks)
     return kBadArgument;
   DeviceGuard guard(a->device);
   if (guard.status()) return guard.status();

@@ -20,6 +20,7 @@ enum Type : int { kFloat32 = 0, kBFloat16 = 1, kFloat16 = 2 };
 
 constexpr int kBadArgument = -1;
 
+constexpr int kMaxBlocks = (1 << 24) - 1;  // of 256 threads, in one dimension
 constexpr int kMaxHeadDim = 128;
 constexpr int kMaxTokens = 1 << 24;
 constexpr int64_t kMaxTokenStride = 1 << 24;
@@ -28,6 +29,7 @@ constexpr int kMaxTop = 32;
 constexpr int kMaxVocab = 1 << 30;
 constexpr int kMaxVocabParts = 64;
 constexpr int kMaxNormDim = 16384;
+constexpr int kMaxGates = 1 << 21;
 
 struct AttentionArgs {
   const bf16 *q, *k, *v;  // [batch][heads][tokens][dim] by strides, dim dense

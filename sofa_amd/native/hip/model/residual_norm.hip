@@ -149,8 +149,10 @@ __global__ __launch_bounds__(kBlock<TEAM>) void norm_backward_kernel(
   const int lane = threadIdx.x % TEAM, team = threadIdx.x / TEAM;
   const int64_t group = blockIdx.x / a.group_blocks;
   const int64_t part = blockIdx.x % a.group_blocks;
-  const int64_t first = group * a.group_rows + a.group_rows * part / a.group_blocks;
-  const int64_t last = group * a.group_rows + a.group_rows * (part + 1) / a.group_blocks;
+  const int64_t first =
+      group * a.group_rows + a.group_rows * part / a.group_blocks;
+  const int64_t last =
+      group * a.group_rows + a.group_rows * (part + 1) / a.group_blocks;
   const float inv_dim = 1.f / (float) a.dim;
   int parity = 0;
 
@@ -439,7 +441,8 @@ struct Backward {
 };
 
 bool sound(const NormArgs* a) {
-  return a && a->rows > 0 && a->rows <= INT32_MAX && a->dim > 0 && a->dim <= kMaxNormDim &&
+  return a && a->rows > 0 && a->rows <= INT32_MAX && a->dim > 0 &&
+         a->dim <= kMaxNormDim &&
          a->group_rows > 0 && a->rows % a->group_rows == 0 && a->x &&
          a->weight && (a->branch || !(a->post || a->gate));
 }
@@ -460,7 +463,8 @@ int sofa_norm_forward(const sofa_model::NormArgs* a) {
 int sofa_norm_backward(const sofa_model::NormArgs* a) {
   using namespace sofa_model;
   if (!sound(a) || !a->dx || !(a->dr || a->dy) || a->group_blocks < 1 ||
-      a->rows / a->group_rows > INT32_MAX / a->group_blocks)
+      a->rows / a->group_rows > kMaxGates ||
+      a->rows / a->group_rows * a->group_blocks > kMaxBlocks / 4)
     return kBadArgument;
   if ((a->dweight || a->dpost || a->dgate) && !a->partial) return kBadArgument;
   if ((a->dpost && !a->post) || (a->dgate && !a->gate)) return kBadArgument;

@@ -28,6 +28,18 @@ __device__ __forceinline__ int64_t place(int64_t row, int64_t inner,
   return row / inner * outer_stride + row % inner * inner_stride;
 }
 
+// A launch has less than 2^32 threads in a dimension, so rows go on in the next.
+constexpr int64_t kRowsInX = 1 << 22;
+
+__device__ __forceinline__ int64_t row_of(const LogprobArgs& a) {
+  return blockIdx.y * kRowsInX + blockIdx.x / a.parts;
+}
+
+inline dim3 grid_of(const LogprobArgs& a) {
+  return dim3((unsigned) (a.rows < kRowsInX ? a.rows : kRowsInX) * a.parts,
+              (unsigned) ((a.rows + kRowsInX - 1) / kRowsInX));
+}
+
 struct Sums {
   float m, s, a;
 };
@@ -270,7 +282,8 @@ __global__ __launch_bounds__(kThreads) void logprob_kernel(LogprobArgs a) {
   __shared__ float sums[kWaves][3];
   __shared__ uint64_t lists[TOP ? kWaves * kListSize : 1];
   const int lane = threadIdx.x % kWave, wave = threadIdx.x / kWave;
-  const int64_t row = blockIdx.x / a.parts;
+  const int64_t row = row_of(a);
+  if (row >= a.rows) return;
   const int part = blockIdx.x % a.parts;
   const T* x = static_cast<const T*>(a.logits) +
                place(row, a.inner, a.outer_stride, a.inner_stride);
@@ -392,7 +405,8 @@ __global__ __launch_bounds__(kWave) void logprob_join_kernel(LogprobArgs a) {
 template <typename T>
 __global__ __launch_bounds__(kThreads) void logprob_backward_kernel(
     LogprobArgs a) {
-  const int64_t row = blockIdx.x / a.parts;
+  const int64_t row = row_of(a);
+  if (row >= a.rows) return;
   const int part = blockIdx.x % a.parts;
   const T* x = static_cast<const T*>(a.logits) +
                place(row, a.inner, a.outer_stride, a.inner_stride);
@@ -453,7 +467,7 @@ __global__ __launch_bounds__(kThreads) void logprob_backward_kernel(
 template <typename T>
 int forward(const LogprobArgs& a) {
   const hipStream_t stream = static_cast<hipStream_t>(a.stream);
-  const dim3 grid((unsigned) (a.rows * a.parts));
+  const dim3 grid = grid_of(a);
   if (a.top)
     hipLaunchKernelGGL((logprob_kernel<T, true>), grid, dim3(kThreads), 0,
                        stream, a);
@@ -474,7 +488,7 @@ int forward(const LogprobArgs& a) {
 template <typename T>
 int backward(const LogprobArgs& a) {
   hipLaunchKernelGGL(logprob_backward_kernel<T>,
-                     dim3((unsigned) (a.rows * a.parts)), dim3(kThreads), 0,
+                     grid_of(a), dim3(kThreads), 0,
                      static_cast<hipStream_t>(a.stream), a);
   return (int) hipGetLastError();
 }
@@ -486,7 +500,7 @@ bool sound(const LogprobArgs* a) {
          a->parts <= kMaxVocabParts && a->part_size > 0 &&
          (int64_t) a->parts * a->part_size >= a->vocab &&
          (int64_t) (a->parts - 1) * a->part_size < a->vocab &&
-         a->rows <= INT32_MAX / a->parts;
+         a->rows <= INT32_MAX && (a->parts == 1 || a->rows <= kMaxBlocks / a->parts);
 }
 
 }  // namespace

@@ -27,8 +27,10 @@ _TYPES = (torch.float32, torch.bfloat16, torch.float16)
 
 MAX_HEAD_DIM = 128
 MAX_TOKENS = 1 << 24
+_MAX_BLOCKS = (1 << 24) - 1  # 128 tokens of one head each
 MAX_TOP = 32
 MAX_NORM_DIM = 16384
+_MAX_GATES = 1 << 21
 MAX_VOCAB = 1 << 30
 
 _module = None
@@ -75,7 +77,7 @@ def attention(
     where kv_heads divides heads and query head i reads key head
     i // (heads // kv_heads).  All are bfloat16; dim is a multiple of 8 up to
     128; any strides (rows that are not dense or not at multiples of 16 bytes
-    are copied first).  scale is above 0, 1 / sqrt(dim) if not given.
+    are copied first).  scale is above 0 (1e-18 to 1e18), 1 / sqrt(dim) if not given.
 
     causal: token i sees tokens 0..i, otherwise all.  lengths: int32 (batch,),
     the valid tokens at the front of each sequence, taken as within 0..tokens;
@@ -88,6 +90,7 @@ def attention(
     value in long sequences.
 
     Returns (batch, heads, tokens, dim), laid out as (batch, tokens, heads, dim).
+    For a backward pass q, k, v and twice the size of the result are kept.
     """
     for name, t in (("q", q), ("k", k), ("v", v)):
         if t.dim() != 4:
@@ -102,12 +105,12 @@ def attention(
         raise ValueError(f"attention: {heads} heads cannot share {k.shape[1]} key heads")
     if dim < 8 or dim % 8 or dim > MAX_HEAD_DIM:
         raise ValueError(f"attention: dim has to be a multiple of 8 up to {MAX_HEAD_DIM}, got {dim}")
-    if tokens > MAX_TOKENS or batch * heads * -(-tokens // 128) > 2**28 - 1:
+    if tokens > MAX_TOKENS or batch * heads * -(-tokens // 128) > _MAX_BLOCKS:
         raise ValueError(f"attention: {tuple(q.shape)} is too large")
     if scale is None:
         scale = 1.0 / math.sqrt(dim)
-    elif not (math.isfinite(scale) and scale > 0):
-        raise ValueError(f"attention: scale has to be above 0 and finite, got {scale}")
+    elif not 1e-18 <= scale <= 1e18:
+        raise ValueError(f"attention: scale has to be within 1e-18..1e18, got {scale}")
     if lengths is not None:
         if lengths.dtype != torch.int32:
             raise TypeError(f"attention: lengths has to be int32, got {lengths.dtype}")
@@ -224,10 +227,12 @@ def residual_norm(
         raise TypeError(f"residual_norm: a branch of {branch_dtype} onto {x.dtype} is not built")
     if out_dtype not in (x.dtype, branch_dtype):
         raise TypeError(f"residual_norm: out_dtype has to be {x.dtype} or {branch_dtype}, got {out_dtype}")
-    if not (math.isfinite(eps) and eps >= 0):
-        raise ValueError(f"residual_norm: eps has to be 0 or more, got {eps}")
-    if not math.isfinite(scale):
-        raise ValueError(f"residual_norm: scale has to be finite, got {scale}")
+    if not 0 <= eps <= 1e30:
+        raise ValueError(f"residual_norm: eps has to be within 0..1e30, got {eps}")
+    if not abs(scale) <= 1e30:
+        raise ValueError(f"residual_norm: scale has to be within -1e30..1e30, got {scale}")
+    if gate is not None and gate.numel() // dim > _MAX_GATES:
+        raise ValueError(f"residual_norm: {gate.numel() // dim} gates are too many")
     if x.numel() // dim > 2**31 - 1:
         raise ValueError(f"residual_norm: {x.numel() // dim} rows are too many")
     _on_gpu("residual_norm", x, branch=branch, weight=weight, post_weight=post_weight, gate=gate)

@@ -55,6 +55,8 @@ def _qkv(b=1, h=4, kv=2, t=5, d=16, dtype=BF16):
     (lambda a: a.update(scale=0.0), ValueError),
     (lambda a: a.update(scale=-1.0), ValueError),
     (lambda a: a.update(scale=math.nan), ValueError),
+    (lambda a: a.update(scale=1e300), ValueError),
+    (lambda a: a.update({n: a[n][:1, :, :1].expand(1 << 20, -1, -1, -1) for n in "qkv"}, q=a["q"][:1, :1, :1].expand(1 << 20, 16, 1, 16)), ValueError),
     (lambda a: a.update(lengths=torch.ones(1, dtype=torch.int64)), TypeError),
     (lambda a: a.update(lengths=torch.ones(2, dtype=torch.int32)), ValueError),
     (lambda a: None, ValueError),  # sound, but not on a GPU
@@ -99,6 +101,8 @@ def test_token_logprobs_refuses(logits, tokens, kw, error):
     (dict(out_dtype=torch.float64), TypeError),
     (dict(eps=-1.0), ValueError),
     (dict(scale=math.inf), ValueError),
+    (dict(scale=1e39), ValueError),
+    (dict(eps=math.nan), ValueError),
     (dict(), ValueError),  # not on a GPU
 ])
 def test_residual_norm_refuses(change, error):
@@ -501,6 +505,22 @@ def test_token_logprobs_far_rows():
 
 
 @pytest.mark.gpu
+def test_token_logprobs_many_rows():
+    """More rows than one dimension of a launch holds."""
+    rows = (1 << 22) * 4 + 5
+    x = (torch.arange(rows, device="cuda") % 7).to(BF16)[:, None] * torch.arange(3, device="cuda", dtype=BF16)
+    x.requires_grad_()
+    ids = torch.full((rows,), 2, device="cuda")
+    lp = kernels.token_logprobs(x, ids).logprob
+    want = torch.log_softmax(x.detach()[:7].double(), -1)[:, 2]
+    # sums of three terms, a logarithm and a difference, of values up to 12
+    assert (lp.double() - want[torch.arange(rows, device="cuda") % 7]).abs().max() <= 64 * STEP
+    (dx,) = torch.autograd.grad(lp, x, torch.ones_like(lp))
+    exact = torch.eye(3, device="cuda", dtype=torch.float64)[2] - torch.softmax(x.detach()[:7].double(), -1)
+    assert (dx.double() - exact[torch.arange(rows, device="cuda") % 7]).abs().max() <= U[BF16] + 64 * STEP
+
+
+@pytest.mark.gpu
 def test_token_logprobs_differences():
     x, tokens, g, h = logits_case(4, 300, FP32, seed=9, std=1.0)
     leaf = x.clone().requires_grad_()
@@ -760,6 +780,34 @@ def test_on_a_stream_of_its_own():
         got = _run(*inputs)
     stream.synchronize()
     assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+@pytest.mark.gpu
+def test_two_threads_at_once():
+    """Each on a stream of its own; what they compute is their own."""
+    import threading
+
+    want = [_run(*_step(seed)) for seed in (1, 2)]
+    inputs = [_step(seed) for seed in (1, 2)]
+    torch.cuda.synchronize()
+    got = [[], []]
+
+    def work(i):
+        stream = torch.cuda.Stream()
+        with torch.cuda.stream(stream):
+            for _ in range(5):
+                got[i].append(_run(*inputs[i]))
+        stream.synchronize()
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    for i in range(2):
+        assert len(got[i]) == 5
+        for run in got[i]:
+            assert all(torch.equal(a, b) for a, b in zip(run, want[i]))
 
 
 @pytest.mark.gpu
