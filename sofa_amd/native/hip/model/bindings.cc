@@ -302,7 +302,7 @@ LogprobArgs logprob_args(const Tensor& logits, Tensor& tokens, int64_t top,
 }
 
 struct LogprobResults {
-  Tensor logprob, entropy, lse, ids, values;
+  Tensor logprob, entropy, norm, ids, values;
 };
 
 LogprobResults logprob_forward(const Tensor& logits, Tensor& tokens, int64_t top,
@@ -312,7 +312,7 @@ LogprobResults logprob_forward(const Tensor& logits, Tensor& tokens, int64_t top
   const auto longs = tokens.options();
   LogprobResults r{at::empty(tokens.sizes(), floats),
                    at::empty(tokens.sizes(), floats),
-                   at::empty(tokens.sizes(), floats), {}, {}};
+                   at::empty({a.rows, 2}, floats), {}, {}};
   Tensor part_sums, part_top;
   if (top) {
     std::vector<int64_t> shape = tokens.sizes().vec();
@@ -326,7 +326,7 @@ LogprobResults logprob_forward(const Tensor& logits, Tensor& tokens, int64_t top
   }
   a.logprob = ptr<float>(r.logprob);
   a.entropy = ptr<float>(r.entropy);
-  a.lse = ptr<float>(r.lse);
+  a.norm = ptr<float>(r.norm);
   a.top_ids = ptr<int64_t>(r.ids);
   a.top_logprobs = ptr<float>(r.values);
   a.part_sums = ptr<float>(part_sums);
@@ -343,7 +343,7 @@ struct TokenLogprobs : torch::autograd::Function<TokenLogprobs> {
     Tensor tokens = tokens_in;
     const LogprobResults r = logprob_forward(logits, tokens, top, ignore_index);
     ctx->set_materialize_grads(false);
-    ctx->save_for_backward({logits, tokens, r.entropy, r.lse});
+    ctx->save_for_backward({logits, tokens, r.entropy, r.norm});
     ctx->saved_data["ignore_index"] = ignore_index;
     if (!top) return {r.logprob, r.entropy};
     ctx->mark_non_differentiable({r.ids, r.values});
@@ -353,7 +353,7 @@ struct TokenLogprobs : torch::autograd::Function<TokenLogprobs> {
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
     if (!grads[0].defined() && !grads[1].defined()) return variable_list(4);
     const variable_list saved = ctx->get_saved_variables();
-    const Tensor &logits = saved[0], &entropy = saved[2], &lse = saved[3];
+    const Tensor &logits = saved[0], &entropy = saved[2];
     Tensor tokens = saved[1];
     LogprobArgs a = logprob_args(logits, tokens, 0,
                                  ctx->saved_data["ignore_index"].toInt());
@@ -368,7 +368,7 @@ struct TokenLogprobs : torch::autograd::Function<TokenLogprobs> {
     const Tensor dlogits =
         at::empty_like(logits, at::MemoryFormat::Contiguous);
     a.logprob = a.entropy = ptr<float>(entropy);
-    a.lse = ptr<float>(lse);
+    a.norm = ptr<float>(saved[3]);
     a.dlogprob = ptr<float>(g);
     a.dentropy = ptr<float>(h);
     a.dlogits = ptr(dlogits);

@@ -51,7 +51,8 @@ struct AttentionArgs {
 struct LogprobArgs {
   const void* logits;
   const int64_t* tokens;
-  float *logprob, *entropy, *lse;
+  float *logprob, *entropy;
+  float* norm;         // [rows][2]: the largest logit, log of the sum relative to it
   int64_t* top_ids;    // [rows][top], or null
   float* top_logprobs;
   // when parts > 1: (m, s, a) and the top candidates of each part of a row

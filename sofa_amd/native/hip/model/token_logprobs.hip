@@ -6,8 +6,10 @@
 //   s = sum e^(x - m),   a = sum e^(x - m) (x - m)
 // and moves both to a new maximum m' = m + t:  a' = e^-t (a - t s),
 // s' = e^-t s.  Joined over the row:
-//   lse = m + log s,  logprob = x_token - lse,  entropy = log s - a / s.
-// Gradient, with p = e^(x - lse), g and h the gradients of the two results:
+//   log p = (x - m) - log s,  entropy = log s - a / s,
+// where m and log s stay apart: next to a large m (a row of the type's lowest
+// values) their sum would lose log s.
+// Gradient, with p = e^(log p), g and h the gradients of the two results:
 //   dx_j = g (1[j = token] - p_j) - h p_j (log p_j + entropy)
 //
 // What bounds it is reading the logits.  A row goes to one workgroup, or, when
@@ -49,8 +51,9 @@ __device__ __forceinline__ Sums join(Sums x, Sums y) {
   Sums r;
   r.m = fmaxf(x.m, y.m);
   const float base = r.m == -INFINITY ? 0.f : r.m;
-  // max() keeps a part of -inf from 0 * -inf
-  const float tx = fmaxf(x.m - base, -1e30f), ty = fmaxf(y.m - base, -1e30f);
+  // max() keeps a part of -inf, or of the type's lowest value, from 0 * -inf
+  // (or an overflow); e^-1e4 is 0 already
+  const float tx = fmaxf(x.m - base, -1e4f), ty = fmaxf(y.m - base, -1e4f);
   const float ex = exp2_fast(tx * kLog2e), ey = exp2_fast(ty * kLog2e);
   r.s = x.s * ex + y.s * ey;
   r.a = ex * (x.a + tx * x.s) + ey * (y.a + ty * y.s);
@@ -74,7 +77,7 @@ __device__ __forceinline__ float take(Sums& t, const float (&x)[8]) {
 #pragma unroll
   for (int j = 1; j < 8; ++j) most = fmaxf(most, x[j]);
   if (most > t.m) {
-    const float step = fmaxf(t.m - most, -1e30f);
+    const float step = fmaxf(t.m - most, -1e4f);
     const float e = exp2_fast(step * kLog2e);
     t.a = e * (t.a + step * t.s);
     t.s *= e;
@@ -86,7 +89,7 @@ __device__ __forceinline__ float take(Sums& t, const float (&x)[8]) {
     const float d = x[j] - base;
     const float e = exp2_fast(d * kLog2e);
     t.s += e;
-    t.a += e * fmaxf(d, -1e30f);
+    t.a += e * fmaxf(d, -1e4f);
   }
   return most;
 }
@@ -124,8 +127,8 @@ __device__ __forceinline__ void wave_sync() {
 // Each wave collects the candidates that reach a threshold: at first the
 // `top`-th best of what its lanes have each seen best in their first loads,
 // which at least `top` logits reach and, in random order, about one in a
-// hundred.  A list of more than 128 is cut to its best `top`, and the last of
-// those is the threshold from then on: a row of 128256 takes one or two such
+// hundred.  A list of more than 2 top + 16 is cut to its best `top`, and the last
+// of those is the threshold from then on: a row of 128256 takes a few such
 // cuts.  In the worst (rising) order every step fills the list, which costs
 // time but no result.
 constexpr int kListSize = 1024;
@@ -220,14 +223,21 @@ __device__ __forceinline__ void keep_best(Best& b) {
 __device__ __forceinline__ void offer(Best& b, const float (&x)[8], float most,
                                       bool all, int first, int n) {
   if (!__ballot(n > 0 && (most >= b.floor || all))) return;
+  uint32_t may = 0;
 #pragma unroll
-  for (int j = 0; j < 8; ++j) {
-    const bool may = j < n && (x[j] >= b.floor || all);
-    if (!__ballot(may)) continue;
-    const uint64_t c = candidate(x[j], first + j);
+  for (int j = 0; j < 8; ++j)
+    may |= (j < n && (x[j] >= b.floor || all) ? 1u : 0u) << j;
+  // one of each lane's at a time: rarely more than twice in a row
+  while (__ballot(may != 0)) {
+    const int pick = __ffs(may) - 1;
+    float value = x[0];
+#pragma unroll
+    for (int j = 1; j < 8; ++j) value = pick == j ? x[j] : value;
+    const uint64_t c = candidate(value, first + pick);
     append(b, c, may && c >= b.least);
+    may &= may - 1;
   }
-  if (b.count > 2 * kWave) keep_best(b);
+  if (b.count > 2 * b.top + 16) keep_best(b);
 }
 
 // The best candidate of 8 logits of which n are there, or `most`
@@ -247,7 +257,6 @@ __device__ __forceinline__ void finish(const LogprobArgs& a, int64_t row,
   const float log_s = log2_fast(t.s) * kLn2;
   // a row without one allowed token: no distribution, and no NaN either
   const bool empty = t.s == 0.f;
-  const float lse = empty ? -INFINITY : t.m + log_s;
   const int64_t token =
       a.tokens[place(row, a.inner, a.token_outer_stride, a.token_inner_stride)];
   float logprob = 0.f;
@@ -264,7 +273,8 @@ __device__ __forceinline__ void finish(const LogprobArgs& a, int64_t row,
   }
   a.logprob[row] = logprob;
   a.entropy[row] = empty ? 0.f : log_s - t.a / t.s;
-  a.lse[row] = lse;
+  a.norm[row * 2] = empty ? -INFINITY : t.m;
+  a.norm[row * 2 + 1] = log_s;
 }
 
 __device__ __forceinline__ void put_top(const LogprobArgs& a, int64_t row,
@@ -413,7 +423,8 @@ __global__ __launch_bounds__(kThreads) void logprob_backward_kernel(
   T* dx = static_cast<T*>(a.dlogits) + row * a.vocab;
   const int begin = part * a.part_size;
   const int end = min(a.vocab, begin + a.part_size);
-  const float lse = a.lse[row], entropy = a.entropy[row];
+  const float m = a.norm[row * 2], log_s = a.norm[row * 2 + 1];
+  const float entropy = a.entropy[row];
   int64_t token =
       a.tokens[place(row, a.inner, a.token_outer_stride, a.token_inner_stride)];
   float g = 0.f, h = 0.f;
@@ -424,7 +435,7 @@ __global__ __launch_bounds__(kThreads) void logprob_backward_kernel(
     h = a.dentropy[place(row, a.inner, a.grad2_outer_stride,
                          a.grad2_inner_stride)];
   // nothing to pass on, or an empty row: zeros, and nothing is read
-  const bool zero = (g == 0.f && h == 0.f) || lse == -INFINITY;
+  const bool zero = (g == 0.f && h == 0.f) || m == -INFINITY;
   // dx = g 1[token] - p (g + h entropy + h log p)
   const float base = g + h * entropy;
 
@@ -433,10 +444,10 @@ __global__ __launch_bounds__(kThreads) void logprob_backward_kernel(
   auto gradient = [&](float (&v)[8], int first) {
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
-      const float logp = v[j] - lse;
+      const float logp = (v[j] - m) - log_s;
       const float p = exp2_fast(logp * kLog2e);
       // a masked logit has p = 0 and log p = -inf
-      float d = -p * (base + h * fmaxf(logp, -1e30f));
+      float d = -p * (base + h * fmaxf(logp, -1e4f));
       if (first + j == token) d += g;
       v[j] = zero ? 0.f : d;
     }
@@ -494,7 +505,7 @@ int backward(const LogprobArgs& a) {
 }
 
 bool sound(const LogprobArgs* a) {
-  return a && a->logits && a->tokens && a->logprob && a->entropy && a->lse &&
+  return a && a->logits && a->tokens && a->logprob && a->entropy && a->norm &&
          a->rows > 0 && a->inner > 0 && a->vocab > 0 && a->vocab <= kMaxVocab &&
          a->parts > 0 &&
          a->parts <= kMaxVocabParts && a->part_size > 0 &&

@@ -6,7 +6,8 @@
 
 All three are differentiable (first derivatives), run on the current stream of
 their tensors' device, allocate what they return and nothing that outlives the
-call, give the same bits for the same inputs, and can be captured into a graph.
+call, give the same bits for the same inputs, and can be captured into a graph
+(a backward pass, as always with torch, while no eager graph of its leaves lives).
 They need tensors on a GPU: there is no other path, and a missing library is an
 error.  Wrong arguments raise TypeError (types) or ValueError (shapes, values).
 

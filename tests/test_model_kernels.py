@@ -436,6 +436,14 @@ def test_token_logprobs_special_rows(rows):
     tokens[4], x[5] = -100, -math.inf
     tokens[5] = -100
     check_logprobs(x, tokens, 3, g, h)
+    # masked with the type's lowest value in place of -inf, a whole row too; gradients of any size
+    for t in (FP32, BF16, FP16):
+        low = torch.finfo(t).min
+        y = x.masked_fill(x == -math.inf, low).to(t)
+        y[2], tokens[2] = low, 7
+        check_logprobs(y, tokens, 3, g, h)
+        check_logprobs(y, tokens, 0, None, h * (2.0**30 if t is FP32 else 1.0))
+    x[2], tokens[2] = x[7], 3
     # what has no value: NaN in that row and nowhere else
     before = kernels.token_logprobs(x, tokens, top=3)
     x[6, 2000], x[7, 5] = math.nan, math.inf
