@@ -42,6 +42,7 @@
 namespace sofa_model {
 namespace {
 
+typedef bf16 bf16x2 __attribute__((ext_vector_type(2)));
 typedef bf16 bf16x4 __attribute__((ext_vector_type(4)));
 typedef bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef short shortx4 __attribute__((ext_vector_type(4)));
@@ -160,6 +161,16 @@ __device__ __forceinline__ bf16x8 rest_of(const floatx16& d, int part,
 
 __device__ __forceinline__ floatx16 mfma(bf16x8 a, bf16x8 b, floatx16 c) {
   return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
+}
+
+// sum + the 8 values
+__device__ __forceinline__ float add_all(bf16x8 x, float sum) {
+  const bf16x2 one = {(bf16) 1.f, (bf16) 1.f};
+#pragma unroll
+  for (int j = 0; j < 4; ++j)
+    sum = __builtin_amdgcn_fdot2_f32_bf16(bf16x2{x[2 * j], x[2 * j + 1]}, one,
+                                          sum, false);
+  return sum;
 }
 
 // A row's elements as B operands, straight from memory; zeros where there are
@@ -295,6 +306,10 @@ __global__ __launch_bounds__(kThreads, 2) void attention_forward_kernel(
                    (int64_t) row * a.q_stride[2],
                row < n, a.dim);
   floatx16 acc[DP / 32] = {};
+  // l sums what 16 bits leave of the probabilities, since it divides their
+  // product: the weights are 1 together then. (Summed before they are rounded, a
+  // row with one large probability is off by all of its rounding, and dP - delta,
+  // almost 0 there, by more than itself.) lse takes the same l, 2^-8 off at most.
   float m = -INFINITY, l = 0.f;
   const float scale = a.scale * kLog2e;
 
@@ -338,17 +353,15 @@ __global__ __launch_bounds__(kThreads, 2) void attention_forward_kernel(
 #pragma unroll
       for (int b = 0; b < DP / 32; ++b) acc[b] *= fade;
     }
-    float sum = 0.f;
 #pragma unroll
     for (int i = 0; i < 32; ++i) {
       const float p = exp2_fast(s[i / 16][i % 16] * scale - m);
       s[i / 16][i % 16] = p;
-      sum += p;
     }
-    l += sum;
 #pragma unroll
     for (int p = 0; p < 4; ++p) {
       const bf16x8 prob = rounded(s[p / 2], p % 2);
+      l = add_all(prob, l);
 #pragma unroll
       for (int b = 0; b < DP / 32; ++b)
         acc[b] = mfma(column_operand<DP>(v_tile, p * 16, b), prob, acc[b]);

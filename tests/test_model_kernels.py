@@ -185,13 +185,15 @@ def attention_64(q, k, v, do, lengths, causal, scale):
             # and one below 2^-126 is 0: exp2 flushes it, an absolute error of up to 2^-126 in each P,
             # which dS = P (dP - delta) takes times |dP - delta|, and bf16 flushes dS at 2^-126 itself
             flush = 2.0**-126
-            eP = P * (u + e) + flush  # rounded to bf16 for its product
-            eO = (u + 2 * e) * (P @ V.abs()) + n * STEP * (P @ V.abs()) + flush * V.abs().sum(0)
+            # P is rounded to bf16 for its product (u), and what it is divided by, and lse, are sums of
+            # such roundings (u again)
+            eP = P * (2 * u + e) + flush
+            eO = (2 * u + 2 * e) * (P @ V.abs()) + n * STEP * (P @ V.abs()) + flush * V.abs().sum(0)
             oO = eO + u * (O.abs() + eO)
             # delta is of o and of what its rounding took off, 16 bits in all
             edelta = (G.abs() * (eO + u * u * O.abs())).sum(-1, keepdim=True) + d * STEP * (G.abs() * O.abs()).sum(-1, keepdim=True)
             edP = d * STEP * (G.abs() @ V.abs().t())
-            edS = flush * ((dP - (G * O).sum(-1, keepdim=True)).abs() + 1) + u * dS.abs() + (1 + u) * (e * dS.abs() + P * (1 + e) * (edelta + edP + 2 * STEP * dP.abs()))
+            edS = flush * ((dP - (G * O).sum(-1, keepdim=True)).abs() + 1) + u * dS.abs() + (1 + u) * ((u + e) * dS.abs() + P * (1 + e) * (edelta + edP + 2 * STEP * dP.abs()))
             value["o"][i, h, :n], bound["o"][i, h, :n] = O, oO
             for name, at, x, ex in (
                 ("dq", h, scale * dS @ K, scale * (edS + n * STEP * dS.abs()) @ K.abs()),
