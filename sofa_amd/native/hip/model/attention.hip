@@ -449,8 +449,10 @@ __global__ __launch_bounds__(kThreads, 2) void attention_dq_kernel(
   }
   const int64_t at = (int64_t) bh * a.tokens + row;
   if (row < a.tokens && h == 0) a.delta[at] = delta;
-  // +inf makes every probability of a row without keys 0
-  const float lse = valid ? a.lse[at] : INFINITY;
+  // +inf makes every probability of a row without keys 0; and with one key alone
+  // dS is 0, not what roundings leave of dP - delta
+  const bool alone = n == 1 || (CAUSAL && row == 0);
+  const float lse = valid && !alone ? a.lse[at] : INFINITY;
   floatx16 acc[DP / 32] = {};
   const float scale = a.scale * kLog2e;
 
@@ -699,18 +701,19 @@ attention_dkv_kernel(AttentionArgs a) {
   __syncthreads();  // the tiles are not read any more
   bf16* stage = tiles_of[0][0] + wave * 32 * DP;
   const int rows = a.tokens - wave_key;
+  const bool has_dk = valid && n > 1;  // dS is 0 for one key alone
   if (a.key_parts > 1) {
     const int64_t size = (int64_t) a.batch * a.kv_heads * a.tokens * a.dim;
     float* out = a.partial + part * 2 * size +
                  ((int64_t) bh * a.tokens + wave_key) * a.dim;
-    store_rows<DP>(stage, out, rows, a.dim, dk, valid);
+    store_rows<DP>(stage, out, rows, a.dim, dk, has_dk);
     store_rows<DP>(stage, out + size, rows, a.dim, dv, valid);
     return;
   }
   store_rows<DP>(stage,
                  a.dk + batch * a.dk_stride[0] + kv_head * a.dk_stride[1] +
                      (int64_t) wave_key * a.dk_stride[2],
-                 a.dk_stride[2], rows, a.dim, dk, a.scale, valid);
+                 a.dk_stride[2], rows, a.dim, dk, a.scale, has_dk);
   store_rows<DP>(stage,
                  a.dv + batch * a.dv_stride[0] + kv_head * a.dv_stride[1] +
                      (int64_t) wave_key * a.dv_stride[2],

@@ -258,6 +258,21 @@ def test_attention_padded(t, d, lengths, causal):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("causal", [True, False])
+@pytest.mark.parametrize("t, d, lengths", [(1, 16, None), (1, 128, None), (40, 64, [1, 1]), (300, 128, [1, 300])])
+def test_attention_one_key(t, d, lengths, causal):
+    """A token that sees one key passes nothing on to its query and that key."""
+    q, k, v, do = attention_case(2, 4, 2, t, d, seed=13, std=3.0)
+    valid = None if lengths is None else torch.tensor(lengths, dtype=torch.int32, device="cuda")
+    _, (dq, dk, _) = check_attention(q, k, v, do, valid, causal)
+    assert not dq[0, :, :1].any()
+    if t == 1 or lengths[0] == 1:
+        assert not dq[0].any() and not dk[0].any()
+    if causal:
+        assert not dq[:, :, 0].any()
+
+
+@pytest.mark.gpu
 def test_attention_large_scores():
     """Scores in the hundreds: a softmax that is almost a choice; a scale of the caller's."""
     check_attention(*attention_case(1, 2, 1, 200, 64, std=8.0), scale=0.2)
