@@ -53,7 +53,7 @@ constexpr int kThreads = 256;
 constexpr int kWaves = 4;
 constexpr int kRows = kWaves * 32;  // rows a workgroup owns
 constexpr int kTile = 64;           // rows of the other side at a time
-constexpr int kShort = 256;         // tokens up to which dS has 16 bits
+constexpr int kShort = 256;         // tokens up to which P and dS have 16 bits
 
 // Where the 8 elements `chunk` of `row` of a tile are in LDS.  A row is 256 or
 // 128 bytes and the banks 256, so one chunk of all rows falls on the same banks;
@@ -282,7 +282,7 @@ __device__ __forceinline__ int valid_tokens(const AttentionArgs& a, int batch) {
   return a.lengths ? min(max(a.lengths[batch], 0), a.tokens) : a.tokens;
 }
 
-template <int DP, bool CAUSAL>
+template <int DP, bool CAUSAL, bool SHORT>
 __global__ __launch_bounds__(kThreads, 2) void attention_forward_kernel(
     AttentionArgs a) {
   __shared__ __align__(16) bf16 k_tiles[2][kTile * DP];
@@ -309,8 +309,9 @@ __global__ __launch_bounds__(kThreads, 2) void attention_forward_kernel(
   // l sums what 16 bits leave of the probabilities, since it divides their
   // product: the weights are 1 together then. (Summed before they are rounded, a
   // row with one large probability is off by all of its rounding, and dP - delta,
-  // almost 0 there, by more than itself.) lse takes the same l, 2^-8 off at most.
-  float m = -INFINITY, l = 0.f;
+  // almost 0 there, by more than itself.) lse takes the same l, 2^-8 off at most;
+  // SHORT: their sum before they are rounded.
+  float m = -INFINITY, l = 0.f, l_exact = 0.f;
   const float scale = a.scale * kLog2e;
 
   int end = block * kRows < n ? n : 0;
@@ -350,12 +351,14 @@ __global__ __launch_bounds__(kThreads, 2) void attention_forward_kernel(
       const float fade = exp2_fast(m - next);
       m = next;
       l *= fade;
+      if (SHORT) l_exact *= fade;
 #pragma unroll
       for (int b = 0; b < DP / 32; ++b) acc[b] *= fade;
     }
 #pragma unroll
     for (int i = 0; i < 32; ++i) {
       const float p = exp2_fast(s[i / 16][i % 16] * scale - m);
+      if (SHORT) l_exact += p;
       s[i / 16][i % 16] = p;
     }
 #pragma unroll
@@ -384,10 +387,11 @@ __global__ __launch_bounds__(kThreads, 2) void attention_forward_kernel(
   }
 
   l += other_half(l);
+  l_exact = SHORT ? l_exact + other_half(l_exact) : l;
   const bool valid = row < n;
   if (row < a.tokens && a.lse && h == 0)
     a.lse[(int64_t) bh * a.tokens + row] =
-        valid ? m + log2_fast(l) : INFINITY;
+        valid ? m + log2_fast(l_exact) : INFINITY;
   __syncthreads();  // the tiles are not read any more
   bf16* stage = k_tiles[0] + wave * 32 * DP;
   const int64_t o_at = batch * a.o_stride[0] + head * a.o_stride[1] +
@@ -401,10 +405,11 @@ __global__ __launch_bounds__(kThreads, 2) void attention_forward_kernel(
 
 // dQ, and delta for the other kernel.
 //
-// SHORT: dS is taken with 16 bits, as its rounding and what that took off. In
-// long rows its rounding is one of many and leaves dQ and dK 1.4 times as far
-// off as their own rounding does; in short ones it was up to 1.6 times. There
-// the products that this adds are not what takes the time.
+// SHORT: dS, and P for dV, are taken with 16 bits, as their rounding and what
+// that took off.  In long rows their rounding is one of many and leaves the
+// gradients 1.4 times as far off as their own rounding does; in short ones it
+// was up to 1.8 times.  There the products that this adds are not what takes
+// the time.
 template <int DP, bool CAUSAL, bool SHORT>
 __global__ __launch_bounds__(kThreads, 2) void attention_dq_kernel(
     AttentionArgs a) {
@@ -666,7 +671,9 @@ attention_dkv_kernel(AttentionArgs a) {
       const bf16x8 ds = rounded(dp[p / 2], p % 2);
 #pragma unroll
       for (int c = 0; c < DP / 32; ++c) {
-        dv[c] = mfma(column_operand<DP>(do_tile, p * 16, c), probs, dv[c]);
+        const bf16x8 douts = column_operand<DP>(do_tile, p * 16, c);
+        dv[c] = mfma(douts, probs, dv[c]);
+        if (SHORT) dv[c] = mfma(douts, rest_of(s[p / 2], p % 2, probs), dv[c]);
         const bf16x8 rows = column_operand<DP>(q_tile, p * 16, c);
         dk[c] = mfma(rows, ds, dk[c]);
         if (SHORT) dk[c] = mfma(rows, rest_of(dp[p / 2], p % 2, ds), dk[c]);
@@ -745,28 +752,50 @@ __global__ __launch_bounds__(kThreads) void attention_join_kernel(
          sum);
 }
 
-template <int DP, bool CAUSAL>
+template <int DP, bool CAUSAL, bool SHORT>
 int forward(const AttentionArgs& a) {
   const int64_t blocks = (a.tokens + kRows - 1) / kRows;
-  hipLaunchKernelGGL((attention_forward_kernel<DP, CAUSAL>),
+  hipLaunchKernelGGL((attention_forward_kernel<DP, CAUSAL, SHORT>),
+                     dim3((unsigned) (blocks * a.batch * a.heads)),
+                     dim3(kThreads), 0, static_cast<hipStream_t>(a.stream), a);
+  return (int) hipGetLastError();
+}
+
+template <int DP, bool CAUSAL>
+int forward(const AttentionArgs& a) {
+  return a.tokens <= kShort ? forward<DP, CAUSAL, true>(a)
+                            : forward<DP, CAUSAL, false>(a);
+}
+
+template <int DP, bool CAUSAL, bool SHORT>
+int dq(const AttentionArgs& a) {
+  const int64_t blocks = (a.tokens + kRows - 1) / kRows;
+  hipLaunchKernelGGL((attention_dq_kernel<DP, CAUSAL, SHORT>),
                      dim3((unsigned) (blocks * a.batch * a.heads)),
                      dim3(kThreads), 0, static_cast<hipStream_t>(a.stream), a);
   return (int) hipGetLastError();
 }
 
 template <int DP, bool CAUSAL, bool SHORT>
-int backward(const AttentionArgs& a) {
+int dkv(const AttentionArgs& a) {
   const int64_t blocks = (a.tokens + kRows - 1) / kRows;
-  hipLaunchKernelGGL((attention_dq_kernel<DP, CAUSAL, SHORT>),
-                     dim3((unsigned) (blocks * a.batch * a.heads)),
-                     dim3(kThreads), 0, static_cast<hipStream_t>(a.stream), a);
-  int status = (int) hipGetLastError();
-  if (status) return status;
   hipLaunchKernelGGL((attention_dkv_kernel<DP, CAUSAL, SHORT>),
                      dim3((unsigned) (blocks * a.batch * a.kv_heads *
                                       a.key_parts)),
                      dim3(kThreads), 0, static_cast<hipStream_t>(a.stream), a);
-  status = (int) hipGetLastError();
+  return (int) hipGetLastError();
+}
+
+template <int DP, bool CAUSAL>
+int backward(const AttentionArgs& a) {
+  const bool is_short = a.tokens <= kShort;
+  // dQ of short heads as well, where it was 1.5 times as far off as its own
+  // rounding leaves it (1.44 from 64 elements on): 83 us in place of 62 at 2 x
+  // 2048 tokens, 32 heads of 16
+  int status = is_short || a.dim <= 32 ? dq<DP, CAUSAL, true>(a)
+                                       : dq<DP, CAUSAL, false>(a);
+  if (status) return status;
+  status = is_short ? dkv<DP, CAUSAL, true>(a) : dkv<DP, CAUSAL, false>(a);
   if (status || a.key_parts == 1) return status;
   const int64_t threads =
       (int64_t) a.batch * a.kv_heads * a.tokens * (a.dim / 8) * 2;
@@ -774,14 +803,6 @@ int backward(const AttentionArgs& a) {
                      dim3((unsigned) ((threads + kThreads - 1) / kThreads)),
                      dim3(kThreads), 0, static_cast<hipStream_t>(a.stream), a);
   return (int) hipGetLastError();
-}
-
-template <int DP>
-int backward(const AttentionArgs& a) {
-  const bool is_short = a.tokens <= kShort;
-  if (a.causal)
-    return is_short ? backward<DP, true, true>(a) : backward<DP, true, false>(a);
-  return is_short ? backward<DP, false, true>(a) : backward<DP, false, false>(a);
 }
 
 bool sound(const AttentionArgs* a) {
@@ -823,7 +844,9 @@ int sofa_attention_backward(const sofa_model::AttentionArgs* a) {
     return kBadArgument;
   DeviceGuard guard(a->device);
   if (guard.status()) return guard.status();
-  return a->dim <= 64 ? backward<64>(*a) : backward<128>(*a);
+  if (a->dim <= 64)
+    return a->causal ? backward<64, true>(*a) : backward<64, false>(*a);
+  return a->causal ? backward<128, true>(*a) : backward<128, false>(*a);
 }
 
 }  // extern "C"
