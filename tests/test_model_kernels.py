@@ -273,6 +273,40 @@ def test_attention_one_key(t, d, lengths, causal):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("causal", [True, False])
+@pytest.mark.parametrize("h, kv, t, d", [(2, 1, 1100, 24), (2, 2, 600, 8), (1, 1, 257, 32), (3, 3, 256, 16)])
+def test_attention_short_heads(h, kv, t, d, causal):
+    check_attention(*attention_case(1, h, kv, t, d, seed=t), causal=causal)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("causal", [True, False])
+@pytest.mark.parametrize("h, kv, t, d", [(2, 2, 32, 16), (4, 1, 100, 64), (8, 1, 256, 128), (2, 1, 255, 40)])
+def test_attention_short_rows_take_more_of_p(h, kv, t, d, causal):
+    """Up to 256 tokens dV is off by its own rounding and little else."""
+    q, k, v, do = attention_case(1, h, kv, t, d, seed=t)
+    (got,) = torch.autograd.grad(kernels.attention(q, k, v, causal=causal), v, do)
+    u, scale, group = U[BF16], 1 / math.sqrt(d), h // kv
+    want = torch.zeros(v.shape, dtype=torch.float64, device="cuda")
+    bound = torch.zeros_like(want)
+    for i in range(h):
+        Q, K, G = (x.detach()[0, j].double() for x, j in ((q, i), (k, i // group), (do, i)))
+        s = scale * Q @ K.t()
+        if causal:
+            s = s.masked_fill(torch.ones(t, t, dtype=torch.bool, device="cuda").triu(1), -math.inf)
+        P = torch.softmax(s, -1)
+        # as in attention_64, but lse is of the sum before any rounding, and P is its rounding and
+        # what that took off, rounded: u * u of it, and 2^-126 in each that is flushed; the sum
+        # takes both of every P
+        size = scale * (Q.abs() @ K.abs().t()).amax()
+        e = STEP * (2 * (d + 4) * size + 2 * s.abs().masked_fill(s == -math.inf, 0).amax() + t / 32 + 32)
+        eP = P * (e + u * u * (1 + e)) + 2 * 2.0**-126
+        want[0, i // group] += P.t() @ G
+        bound[0, i // group] += (eP + 2 * group * t * STEP * P).t() @ G.abs()
+    close(got, want, bound + u * (want.abs() + bound) + TINY[BF16], "dv")
+
+
+@pytest.mark.gpu
 def test_attention_large_scores():
     """Scores in the hundreds: a softmax that is almost a choice; a scale of the caller's."""
     check_attention(*attention_case(1, 2, 1, 200, 64, std=8.0), scale=0.2)
@@ -787,6 +821,53 @@ def test_first_derivatives_only():
         assert torch.equal(first, plain) and first.requires_grad
         with pytest.raises(RuntimeError, match="first derivatives only"):
             first.sum().backward()
+
+
+@pytest.mark.gpu
+def test_recomputed_and_offloaded():
+    """What a backward pass needs may be computed again or come back from host memory, laid out anew."""
+    from torch.autograd.graph import save_on_cpu
+    from torch.utils.checkpoint import checkpoint
+
+    *inputs, g, h, res, w = _step(4)
+    leaves = [t.requires_grad_() for t in (*inputs[:3], inputs[4], res, w)]
+    do, tokens = inputs[3], inputs[5]
+
+    def forward(q, k, v, x, res, w):
+        # logits and tokens in two levels of rows, queries token-major
+        out = kernels.token_logprobs(x.view(20, 15, -1)[:, :13], tokens.view(20, 15)[:, :13])
+        o = kernels.attention(q, k, v)
+        r, y = kernels.residual_norm(res, o.transpose(1, 2).reshape(2, 150, 256), w, out_dtype=BF16)
+        return r, y, out.logprob, out.entropy
+
+    given = (res.detach(), do.transpose(1, 2).reshape(2, 150, 256), *(t.view(20, 15)[:, :13] for t in (g, h)))
+    want = torch.autograd.grad(forward(*leaves), leaves, given)
+    again = torch.autograd.grad(checkpoint(forward, *leaves, use_reentrant=False), leaves, given)
+    with save_on_cpu():
+        results = forward(*leaves)
+    back = torch.autograd.grad(results, leaves, given)
+    for a, b, c in zip(want, again, back):
+        assert torch.equal(a, b) and torch.equal(a, c)
+
+
+@pytest.mark.gpu
+def test_inputs_changed_before_the_backward_pass():
+    """An error, not gradients of other inputs."""
+    q, k, v, do = attention_case(1, 2, 1, 20, 16)
+    lengths = torch.tensor([12], dtype=torch.int32, device="cuda")
+    x, tokens, g, _ = logits_case(3, 50, FP32)
+    x.requires_grad_()
+    res, w = torch.randn(3, 40, device="cuda", requires_grad=True), torch.ones(40, device="cuda", requires_grad=True)
+    for out, leaf, grad, changed in (
+        (kernels.attention(q, k, v, lengths=lengths), q, do, lengths),
+        (kernels.attention(q, k, v), q, do, k),
+        (kernels.token_logprobs(x, tokens).logprob, x, g, tokens),
+        (kernels.residual_norm(res, None, w)[1], res, torch.ones(3, 40, device="cuda"), w),
+    ):
+        with torch.no_grad():
+            changed.mul_(1)
+        with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+            torch.autograd.grad(out, leaf, grad)
 
 
 @pytest.mark.gpu
