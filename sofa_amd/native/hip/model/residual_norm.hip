@@ -232,7 +232,8 @@ __global__ __launch_bounds__(kBlock<TEAM>) void norm_backward_kernel(
       }
     team_sum<TEAM>(sum, smem, parity);
     const float s = rsqrtf(sum[0] * inv_dim + a.eps);
-    const float c = s * s * s * inv_dim * sum[1];
+    // in this order: s^3 leaves 32 bits for rows of 1e13 and more, or 1e-13
+    const float c = s * sum[1] * inv_dim * s * s;
 #pragma unroll
     for (int v = 0; v < VPT; ++v) {
       const int at = (v * TEAM + lane) * 8;
@@ -261,7 +262,7 @@ __global__ __launch_bounds__(kBlock<TEAM>) void norm_backward_kernel(
           for (int j = 0; j < 8; ++j)
             sums[0] += d[v][j] * gate[v][j] * post[v][j] * h[v][j];
         team_sum<TEAM>(sums, smem, parity);
-        ch = sh * sh * sh * inv_dim * sums[0];
+        ch = sh * sums[0] * inv_dim * sh * sh;
       }
 #pragma unroll
       for (int v = 0; v < VPT; ++v) {

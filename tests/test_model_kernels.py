@@ -757,6 +757,30 @@ def test_residual_norm_zero_rows_and_empty():
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("post", [False, True])
+@pytest.mark.parametrize("size, eps", [(1e15, 1e-5), (1e-15, 0.0)])
+def test_residual_norm_far_from_one(size, eps, post):
+    """Rows so large or small that the cube of their norm leaves 32 bits, and its square does not."""
+    g = torch.Generator(device="cuda").manual_seed(9)
+
+    def normal(*s, std=1.0):
+        return torch.randn(*s, generator=g, device="cuda") * std
+
+    x, b = normal(3, 5, 700, std=size), normal(3, 5, 700, std=size)
+    w, p = normal(700), normal(700) if post else None
+    ga = normal(700, std=size) if post else None
+    dy = normal(3, 5, 700)
+    leaves = {n: t.requires_grad_() for n, t in (("dx", x), ("dbranch", b), ("dweight", w), ("dpost", p), ("dgate", ga))
+              if t is not None}
+    r, y = kernels.residual_norm(x, b, w, post_weight=p, gate=ga, eps=eps)
+    want = norm_64(x, b, w, p, ga, 1.0, eps, None, dy)
+    got = {"r": r, "y": y, **dict(zip(leaves, torch.autograd.grad(y, list(leaves.values()), dy)))}
+    for name, t in got.items():
+        value, bound = want[name]
+        close(t, value, bound + U[FP32] * (value.abs() + bound) + TINY[FP32], name)
+
+
+@pytest.mark.gpu
 def test_residual_norm_differences():
     g = torch.Generator(device="cuda").manual_seed(4)
 
