@@ -282,8 +282,12 @@ __device__ __forceinline__ int valid_tokens(const AttentionArgs& a, int batch) {
   return a.lengths ? min(max(a.lengths[batch], 0), a.tokens) : a.tokens;
 }
 
+// Short heads of long rows: four workgroups on a compute unit, at the cost of a
+// register spilled (2 x 4096 tokens, 32/8 heads of 64, no mask: 325 us in place of
+// 340 with three); a few hundred tokens do not fill them, and lose 3 %.
 template <int DP, bool CAUSAL, bool SHORT>
-__global__ __launch_bounds__(kThreads, 2) void attention_forward_kernel(
+__global__ __launch_bounds__(kThreads, DP > 64 ? 2 : SHORT ? 3 : 4)
+void attention_forward_kernel(
     AttentionArgs a) {
   __shared__ __align__(16) bf16 k_tiles[2][kTile * DP];
   __shared__ __align__(16) bf16 v_tiles[2][kTile * DP];
@@ -411,7 +415,8 @@ __global__ __launch_bounds__(kThreads, 2) void attention_forward_kernel(
 // was up to 1.8 times.  There the products that this adds are not what takes
 // the time.
 template <int DP, bool CAUSAL, bool SHORT>
-__global__ __launch_bounds__(kThreads, 2) void attention_dq_kernel(
+__global__ __launch_bounds__(kThreads, DP > 64 ? 2 : 3)
+void attention_dq_kernel(
     AttentionArgs a) {
   __shared__ __align__(16) bf16 k_tiles[2][kTile * DP];
   __shared__ __align__(16) bf16 v_tiles[2][kTile * DP];
@@ -790,7 +795,7 @@ template <int DP, bool CAUSAL>
 int backward(const AttentionArgs& a) {
   const bool is_short = a.tokens <= kShort;
   // dQ of short heads as well, where it was 1.5 times as far off as its own
-  // rounding leaves it (1.44 from 64 elements on): 83 us in place of 62 at 2 x
+  // rounding leaves it (1.44 from 64 elements on): 78 us in place of 62 at 2 x
   // 2048 tokens, 32 heads of 16
   int status = is_short || a.dim <= 32 ? dq<DP, CAUSAL, true>(a)
                                        : dq<DP, CAUSAL, false>(a);
