@@ -131,7 +131,7 @@ __device__ __forceinline__ void wave_sync() {
 // of those is the threshold from then on: a row of 128256 takes a few such
 // cuts.  In the worst (rising) order every step fills the list, which costs
 // time but no result.
-constexpr int kListSize = 1024;
+constexpr int kListSize = 640;  // 2 top + 16, and what 8 logits a lane may add
 constexpr int kPerLane = kListSize / kWave;
 
 struct Best {
@@ -195,24 +195,34 @@ __device__ __forceinline__ void keep_best(Best& b) {
     wave_sync();
   }
   // the place of a candidate is the number of those above it
-  uint64_t mine[2];
-  int rank[2] = {};
-#pragma unroll
-  for (int k = 0; k < 2; ++k) {
-    const int at = k * kWave + lane;
-    mine[k] = at < b.count ? b.list[at] : 0;
-  }
+  if (b.count <= kWave) {
+    const uint64_t mine = lane < b.count ? b.list[lane] : 0;
+    int rank = 0;
 #pragma unroll 8
-  for (int i = 0; i < b.count; ++i) {
-    const uint64_t other = b.list[i];
+    for (int i = 0; i < b.count; ++i) rank += b.list[i] > mine;
+    wave_sync();
+    if (lane < b.count ? rank < b.top : lane < b.top)
+      b.list[lane < b.count ? rank : lane] = mine;
+  } else {
+    uint64_t mine[2];
+    int rank[2] = {};
 #pragma unroll
-    for (int k = 0; k < 2; ++k) rank[k] += other > mine[k];
+    for (int k = 0; k < 2; ++k) {
+      const int at = k * kWave + lane;
+      mine[k] = at < b.count ? b.list[at] : 0;
+    }
+#pragma unroll 8
+    for (int i = 0; i < b.count; ++i) {
+      const uint64_t other = b.list[i];
+#pragma unroll
+      for (int k = 0; k < 2; ++k) rank[k] += other > mine[k];
+    }
+    wave_sync();
+#pragma unroll
+    for (int k = 0; k < 2; ++k)
+      if (k * kWave + lane < b.count && rank[k] < b.top)
+        b.list[rank[k]] = mine[k];
   }
-  wave_sync();
-  if (lane >= b.count && lane < b.top) b.list[lane] = 0;
-#pragma unroll
-  for (int k = 0; k < 2; ++k)
-    if (k * kWave + lane < b.count && rank[k] < b.top) b.list[rank[k]] = mine[k];
   wave_sync();
   if (b.count > b.top) b.count = b.top;
   if (b.count == b.top) b.raise(b.list[b.top - 1]);
@@ -286,9 +296,12 @@ __device__ __forceinline__ void put_top(const LogprobArgs& a, int64_t row,
       t.s == 0.f ? -INFINITY : (x - t.m) - log_s;
 }
 
-// `part` of `parts` of a row.  TOP: with alternatives.
+// `part` of `parts` of a row.  TOP: with alternatives; looking for those leaves
+// memory idle unless the next loads are on their way and there are four workgroups
+// on a compute unit (8192 x 128256 bf16, 5 alternatives: 403 us, without 365; one
+// load after the other 502).
 template <typename T, bool TOP>
-__global__ __launch_bounds__(kThreads) void logprob_kernel(LogprobArgs a) {
+__global__ __launch_bounds__(kThreads, 4) void logprob_kernel(LogprobArgs a) {
   __shared__ float sums[kWaves][3];
   __shared__ uint64_t lists[TOP ? kWaves * kListSize : 1];
   const int lane = threadIdx.x % kWave, wave = threadIdx.x / kWave;
@@ -302,14 +315,16 @@ __global__ __launch_bounds__(kThreads) void logprob_kernel(LogprobArgs a) {
 
   Sums t{-INFINITY, 0.f, 0.f};
   Best best{lists + (TOP ? wave * kListSize : 0), 0, 0, -INFINITY, a.top};
-  constexpr int kLoads = 4;  // vectors in flight a thread
+  constexpr int kLoads = TOP ? 2 : 4;  // vectors a thread loads at a time
   constexpr int kStep = kThreads * 8;
+  constexpr int kStride = kLoads * kStep;
   int at = begin;
-  for (; at + kLoads * kStep <= end; at += kLoads * kStep) {
-    float v[kLoads][8];
+  auto fetch = [&](float (&v)[kLoads][8], int at) {
 #pragma unroll
     for (int k = 0; k < kLoads; ++k)
       load8(x + at + k * kStep + threadIdx.x * 8, v[k]);
+  };
+  auto process = [&](const float (&v)[kLoads][8], int at) {
     if constexpr (TOP) {
       if (at == begin) {
         uint64_t most = 0;
@@ -324,6 +339,29 @@ __global__ __launch_bounds__(kThreads) void logprob_kernel(LogprobArgs a) {
       const float most = take(t, v[k]);
       if constexpr (TOP)
         offer(best, v[k], most, t.s != t.s, at + k * kStep + threadIdx.x * 8, 8);
+    }
+  };
+  if constexpr (TOP) {
+    // the next loads are on their way while candidates are looked at
+    if (at + kStride <= end) {
+      float v[kLoads][8], next[kLoads][8];
+      fetch(v, at);
+      for (; at + 2 * kStride <= end; at += kStride) {
+        fetch(next, at + kStride);
+        process(v, at);
+#pragma unroll
+        for (int k = 0; k < kLoads; ++k)
+#pragma unroll
+          for (int j = 0; j < 8; ++j) v[k][j] = next[k][j];
+      }
+      process(v, at);
+      at += kStride;
+    }
+  } else {
+    for (; at + kStride <= end; at += kStride) {
+      float v[kLoads][8];
+      fetch(v, at);
+      process(v, at);
     }
   }
   for (; at < end; at += kStep) {
@@ -371,9 +409,10 @@ __global__ __launch_bounds__(kThreads) void logprob_kernel(LogprobArgs a) {
     }
     wave_sync();
     Best joined{lists, 0, 0, -INFINITY, a.top};
+    raise_by_lanes(joined, mine[0] > mine[1] ? mine[0] : mine[1]);
 #pragma unroll
     for (int k = 0; k < kWaves * kMaxTop / kWave; ++k)
-      append(joined, mine[k], mine[k] != 0);
+      append(joined, mine[k], mine[k] && mine[k] >= joined.least);
     keep_best(joined);
     if (lane < a.top) {
       if (a.parts == 1)
@@ -401,6 +440,8 @@ __global__ __launch_bounds__(kWave) void logprob_join_kernel(LogprobArgs a) {
     Best best{list, 0, 0, -INFINITY, a.top};
     const uint64_t* in = a.part_top + row * a.parts * a.top;
     const int all = a.parts * a.top;
+    // each part's best come first
+    raise_by_lanes(best, lane < a.parts ? in[lane * a.top] : 0);
     for (int at = 0; at < all; at += kWave) {
       const int i = at + lane;
       const uint64_t c = i < all ? in[i] : 0;
