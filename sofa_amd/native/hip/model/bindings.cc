@@ -203,12 +203,15 @@ struct Attention : torch::autograd::Function<Attention> {
 };
 
 Tensor attention(const Tensor& q_in, const Tensor& k_in, const Tensor& v_in,
-                 const Optional& lengths, double scale, bool causal) {
+                 const Optional& lengths_in, double scale, bool causal) {
   if (recorded({q_in, k_in, v_in}))
-    return Attention::apply(q_in, k_in, v_in, lengths, scale, causal);
+    return Attention::apply(q_in, k_in, v_in, lengths_in, scale, causal);
+  // the arguments hold addresses only: copies live until the launch
+  const Tensor lengths = dense(unpack(lengths_in));
   const Tensor q = rows16(q_in), k = rows16(k_in), v = rows16(v_in);
   const Tensor o = token_major(q);
-  const AttentionArgs a = attention_args(q, k, v, o, {}, {}, dense(unpack(lengths)), scale, causal);
+  const AttentionArgs a =
+      attention_args(q, k, v, o, {}, {}, lengths, scale, causal);
   check(sofa_attention_forward(&a), "attention");
   return o;
 }

@@ -346,6 +346,19 @@ def test_attention_far_offsets():
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("grad", [False, True])
+def test_attention_strided_lengths(grad):
+    """Lengths that are a column of a table of sizes are copied, and the copy lives until it is read."""
+    q, k, v, _ = attention_case(3, 4, 2, 150, 64, seed=17)
+    lengths = torch.tensor([[9, 150, 1], [7, 20, 3], [5, 0, 2]], dtype=torch.int32, device="cuda")[:, 1]
+    assert not lengths.is_contiguous()
+    with torch.set_grad_enabled(grad):
+        got = kernels.attention(q, k, v, lengths=lengths)
+        assert got.requires_grad == grad
+        assert torch.equal(got, kernels.attention(q, k, v, lengths=lengths.clone()))
+
+
+@pytest.mark.gpu
 def test_attention_empty():
     q, k, v = (x.to("cuda").requires_grad_() for x in _qkv(t=0))
     o = kernels.attention(q, k, v)
