@@ -475,8 +475,9 @@ __global__ __launch_bounds__(kThreads) void logprob_backward_kernel(
   if (a.dentropy)
     h = a.dentropy[place(row, a.inner, a.grad2_outer_stride,
                          a.grad2_inner_stride)];
-  // nothing to pass on, or an empty row: zeros, and nothing is read
-  const bool zero = (g == 0.f && h == 0.f) || m == -INFINITY;
+  // nothing to pass on, or an empty row (no sum, while m is -inf in a row of NaN
+  // and -inf too): zeros, and nothing is read
+  const bool zero = (g == 0.f && h == 0.f) || log_s == -INFINITY;
   // dx = g 1[token] - p (g + h entropy + h log p)
   const float base = g + h * entropy;
 

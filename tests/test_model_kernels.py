@@ -526,6 +526,35 @@ def test_token_logprobs_special_rows(rows):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [BF16, FP16, FP32])
+@pytest.mark.parametrize("rows", [8, 600])  # rows in parts, and whole
+def test_token_logprobs_gradients_of_diverged_rows(rows, dtype):
+    """Rows that have no value have no gradient either: NaN, not zeros, which would pass for converged."""
+    x, tokens, g, h = logits_case(rows, 3001, dtype, seed=21)
+    clean = x.clone().requires_grad_()
+    x[1] = math.nan
+    x[2], x[2, 7] = -math.inf, math.nan
+    x[3, 2999] = math.inf
+    x[4, 9] = math.nan
+    x[5], x[6] = math.nan, math.nan
+    tokens[5] = -100
+    g[6], h[6] = 0.0, 0.0
+    x.requires_grad_()
+    keep = torch.ones(rows, dtype=torch.bool, device="cuda")
+    keep[1:7] = False
+    for dlogprob, dentropy in ((g, None), (None, h), (g, h)):
+        (got,), (want,) = (
+            torch.autograd.grad([o for o, d in zip(kernels.token_logprobs(leaf, tokens), (dlogprob, dentropy)) if d is not None],
+                                leaf, [d for d in (dlogprob, dentropy) if d is not None])
+            for leaf in (x, clean))
+        assert got[1:5].isnan().all()
+        # what passes nothing on gives zeros, whatever the row holds
+        assert not got[6].any()
+        assert got[5].isnan().all() if dentropy is not None else not got[5].any()
+        assert torch.equal(got[keep], want[keep])
+
+
+@pytest.mark.gpu
 def test_token_logprobs_views():
     """All but the last position of a batch, a transposed batch, a lone row, three axes."""
     b, t, vocab = 3, 5, 1003
