@@ -472,12 +472,15 @@ __global__ __launch_bounds__(kThreads) void logprob_backward_kernel(
   if (a.dlogprob && token != a.ignore_index)
     g = a.dlogprob[place(row, a.inner, a.grad_outer_stride,
                          a.grad_inner_stride)];
+  // a log probability of what is no token is NaN, and so is the gradient through it
+  const bool wrong = g != 0.f && (token < 0 || token >= a.vocab);
+  if (wrong) g = __uint_as_float(0x7fc00000u);
   if (a.dentropy)
     h = a.dentropy[place(row, a.inner, a.grad2_outer_stride,
                          a.grad2_inner_stride)];
   // nothing to pass on, or an empty row (no sum, while m is -inf in a row of NaN
   // and -inf too): zeros, and nothing is read
-  const bool zero = (g == 0.f && h == 0.f) || log_s == -INFINITY;
+  const bool zero = (g == 0.f && h == 0.f) || (log_s == -INFINITY && !wrong);
   // dx = g 1[token] - p (g + h entropy + h log p)
   const float base = g + h * entropy;
 

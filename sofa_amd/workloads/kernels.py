@@ -151,10 +151,10 @@ def token_logprobs(
 
     A token equal to ignore_index has log probability 0 and passes no gradient
     on; its entropy and alternatives are there all the same.  Any other token
-    outside 0..vocab-1 has log probability NaN.  Logits of -inf are tokens that
-    are not allowed.  A row without an allowed token has log probability -inf,
-    entropy 0 and gradient 0; one with a NaN or +inf has NaN throughout, in its
-    gradient too where one comes in.
+    outside 0..vocab-1 has log probability NaN, and NaN for a gradient that passes
+    through it.  Logits of -inf are tokens that are not allowed.  A row without an
+    allowed token has log probability -inf, entropy 0 and gradient 0; one with a
+    NaN or +inf has NaN throughout, in its gradient too where one comes in.
     Alternatives of equal logits come in the order of their tokens.
     """
     if logits.dim() < 1 or logits.shape[:-1] != tokens.shape:

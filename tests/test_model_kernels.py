@@ -555,6 +555,29 @@ def test_token_logprobs_gradients_of_diverged_rows(rows, dtype):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("rows", [8, 600])
+def test_token_logprobs_gradient_of_what_is_no_token(rows):
+    """Its log probability is NaN and so is the gradient through it; the entropy's is the row's own."""
+    vocab = 3001
+    x, tokens, g, h = logits_case(rows, vocab, FP32, seed=22)
+    x.requires_grad_()
+    wrong = tokens.clone()
+    wrong[1], wrong[2], wrong[3], wrong[4] = vocab, -1, 2**40, -2**40
+    g[4] = 0.0
+    with torch.no_grad():
+        x[3] = -math.inf  # without an allowed token as well
+    keep = torch.ones(rows, dtype=torch.bool, device="cuda")
+    keep[1:4] = False
+    for dentropy in (None, h):
+        outs = [kernels.token_logprobs(x, t)[:1 if dentropy is None else 2] for t in (wrong, tokens)]
+        got, want = (torch.autograd.grad(o, x, (g, h)[:len(o)])[0] for o in outs)
+        assert got[1:4].isnan().all()
+        assert torch.equal(got[keep], want[keep])
+    got, want = (torch.autograd.grad(kernels.token_logprobs(x, t).entropy, x, h)[0] for t in (wrong, tokens))
+    assert torch.equal(got, want)
+
+
+@pytest.mark.gpu
 def test_token_logprobs_views():
     """All but the last position of a batch, a transposed batch, a lone row, three axes."""
     b, t, vocab = 3, 5, 1003
