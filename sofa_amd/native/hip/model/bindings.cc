@@ -59,6 +59,23 @@ Tensor dense(const Tensor& t) {
 
 int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
+at::ScalarType known_type(const Tensor& t) {
+  const at::ScalarType type = t.scalar_type();
+  TORCH_CHECK(type == at::kFloat || type == at::kBFloat16 || type == at::kHalf,
+              "the model kernels have no ", type);
+  return type;
+}
+
+// What a backward pass is given was saved by the forward pass, but hooks on saved
+// tensors may return it laid out anew, which every one of them allows for, or as
+// something else, which is refused.
+void expect(const char* what, const Tensor& t, bool fits, at::ScalarType type,
+            const Tensor& like) {
+  TORCH_CHECK(t.defined() && fits && t.scalar_type() == type &&
+                  t.device() == like.device(),
+              what, " came back from a hook as another tensor than it was");
+}
+
 // Whether autograd will ask for a backward pass
 bool recorded(std::initializer_list<Tensor> tensors) {
   if (!at::GradMode::is_enabled()) return false;
@@ -102,6 +119,15 @@ Tensor token_major(const Tensor& like) {
   const auto s = like.sizes();
   return at::empty_strided(s, {s[2] * s[1] * s[3], s[3], s[1] * s[3], 1},
                            like.options());
+}
+
+// t, or a copy, laid out so
+Tensor as_token_major(const Tensor& t) {
+  const auto s = t.sizes();
+  if (t.strides() == at::IntArrayRef{s[2] * s[1] * s[3], s[3], s[1] * s[3], 1} &&
+      reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0)
+    return t;
+  return token_major(t).copy_(t);
 }
 
 void put_strides(int64_t (&to)[3], const Tensor& t) {
@@ -173,12 +199,29 @@ struct Attention : torch::autograd::Function<Attention> {
 
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
     const variable_list saved = ctx->get_saved_variables();
-    const Tensor &q = saved[0], &k = saved[1], &v = saved[2];
+    const Tensor& like = grads[0];
+    const auto sizes = like.sizes(), kv_sizes = saved[1].sizes();
+    expect("attention: q", saved[0], saved[0].sizes() == sizes, at::kBFloat16, like);
+    expect("attention: k", saved[1],
+           kv_sizes.size() == 4 && kv_sizes[0] == sizes[0] && kv_sizes[1] > 0 &&
+               sizes[1] % kv_sizes[1] == 0 && kv_sizes.slice(2) == sizes.slice(2),
+           at::kBFloat16, like);
+    expect("attention: v", saved[2], saved[2].sizes() == kv_sizes, at::kBFloat16, like);
+    for (int i : {3, 4})
+      expect("attention: o", saved[i], saved[i].sizes() == sizes, at::kBFloat16, like);
+    expect("attention: lse", saved[5], saved[5].sizes() == sizes.slice(0, 3), at::kFloat,
+           like);
+    if (saved[6].defined())
+      expect("attention: lengths", saved[6], saved[6].sizes() == sizes.slice(0, 1),
+             at::kInt, like);
+    const Tensor q = rows16(saved[0]), k = rows16(saved[1]), v = rows16(saved[2]),
+                 o = as_token_major(saved[3]), o_low = as_token_major(saved[4]),
+                 lse = dense(saved[5]), lengths = dense(saved[6]);
     const Tensor dout = rows16(grads[0]);
     const Tensor dq = token_major(q), dk = token_major(k), dv = token_major(v);
-    const Tensor delta = at::empty_like(saved[5]);
-    AttentionArgs a = attention_args(q, k, v, saved[3], saved[4], saved[5],
-                                     saved[6], ctx->saved_data["scale"].toDouble(),
+    const Tensor delta = at::empty_like(lse);
+    AttentionArgs a = attention_args(q, k, v, o, o_low, lse, lengths,
+                                     ctx->saved_data["scale"].toDouble(),
                                      ctx->saved_data["causal"].toBool());
     a.dout = ptr<sofa_model::bf16>(dout);
     a.delta = ptr<float>(delta);
@@ -356,8 +399,20 @@ struct TokenLogprobs : torch::autograd::Function<TokenLogprobs> {
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
     if (!grads[0].defined() && !grads[1].defined()) return variable_list(4);
     const variable_list saved = ctx->get_saved_variables();
-    const Tensor &logits = saved[0], &entropy = saved[2];
     Tensor tokens = saved[1];
+    const Tensor& like = grads[0].defined() ? grads[0] : grads[1];
+    const auto sizes = like.sizes();
+    expect("token_logprobs: logits", saved[0],
+           saved[0].dim() == like.dim() + 1 && saved[0].size(-1) > 0 &&
+               saved[0].sizes().slice(0, like.dim()) == sizes,
+           known_type(saved[0]), like);
+    expect("token_logprobs: tokens", tokens, tokens.sizes() == sizes, at::kLong, like);
+    expect("token_logprobs: entropy", saved[2], saved[2].sizes() == sizes, at::kFloat,
+           like);
+    expect("token_logprobs: norm", saved[3],
+           saved[3].sizes() == at::IntArrayRef{tokens.numel(), 2}, at::kFloat, like);
+    const Tensor logits = logit_rows(saved[0]), entropy = dense(saved[2]),
+                 norm = dense(saved[3]);
     LogprobArgs a = logprob_args(logits, tokens, 0,
                                  ctx->saved_data["ignore_index"].toInt());
     const int64_t axes = tokens.dim();
@@ -371,7 +426,7 @@ struct TokenLogprobs : torch::autograd::Function<TokenLogprobs> {
     const Tensor dlogits =
         at::empty_like(logits, at::MemoryFormat::Contiguous);
     a.logprob = a.entropy = ptr<float>(entropy);
-    a.norm = ptr<float>(saved[3]);
+    a.norm = ptr<float>(norm);
     a.dlogprob = ptr<float>(g);
     a.dentropy = ptr<float>(h);
     a.dlogits = ptr(dlogits);
@@ -488,14 +543,34 @@ struct ResidualNorm : torch::autograd::Function<ResidualNorm> {
     const Tensor dr = grads.size() > 1 ? dense(grads[1]) : Tensor();
     if (!dr.defined() && !dy.defined()) return variable_list(8);
     const variable_list saved = ctx->get_saved_variables();
-    const Tensor &x = saved[0], &weight = saved[2], &post = saved[3],
-                 &gate = saved[4];
+    const Tensor& like = dy.defined() ? dy : dr;
     const auto branch_type =
         (at::ScalarType) ctx->saved_data["branch_type"].toInt();
-    NormArgs a = norm_args(x, saved[1], weight, post, gate,
+    const auto y_type = (at::ScalarType) ctx->saved_data["y_type"].toInt();
+    const auto sizes = like.sizes(), dim = sizes.slice(sizes.size() - 1);
+    expect("residual_norm: x", saved[0], saved[0].sizes() == sizes,
+           dr.defined() ? dr.scalar_type() : known_type(saved[0]), like);
+    if (saved[1].defined())
+      expect("residual_norm: branch", saved[1], saved[1].sizes() == sizes, branch_type,
+             like);
+    expect("residual_norm: weight", saved[2], saved[2].sizes() == dim,
+           known_type(saved[2]), like);
+    if (saved[3].defined())
+      expect("residual_norm: post_weight", saved[3], saved[3].sizes() == dim,
+             known_type(saved[3]), like);
+    if (saved[4].defined())
+      expect("residual_norm: gate", saved[4],
+             saved[4].dim() > 0 && saved[4].size(-1) == dim[0] &&
+                 (saved[4].dim() == 1 || (saved[4].dim() == like.dim() &&
+                                          saved[4].size(0) == sizes[0] &&
+                                          saved[4].numel() == sizes[0] * dim[0])),
+             known_type(saved[4]), like);
+    const Tensor x = dense(saved[0]), branch = dense(saved[1]),
+                 weight = dense(saved[2]), post = dense(saved[3]),
+                 gate = dense(saved[4]);
+    NormArgs a = norm_args(x, branch, weight, post, gate,
                            ctx->saved_data["scale"].toDouble(),
-                           ctx->saved_data["eps"].toDouble(), branch_type,
-                           (at::ScalarType) ctx->saved_data["y_type"].toInt());
+                           ctx->saved_data["eps"].toDouble(), branch_type, y_type);
     const int64_t needed = ctx->saved_data["needed"].toInt();
     const Tensor dx = at::empty_like(x);
     Tensor dbranch, dweight, dpost, dgate, partial;

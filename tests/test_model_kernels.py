@@ -939,6 +939,78 @@ def test_recomputed_and_offloaded():
         assert torch.equal(a, b) and torch.equal(a, c)
 
 
+def _steps_for_hooks():
+    """Each operator's results, the leaves, the gradients that come in, and how many tensors it saves."""
+    q, k, v, do = attention_case(2, 4, 2, 70, 64, seed=8)
+    lengths = torch.tensor([70, 33], dtype=torch.int32, device="cuda")
+    x, tokens, g, h = logits_case(30, 700, BF16, seed=8)
+    x = x.view(6, 5, 700).requires_grad_()
+    tokens, g, h = (t.view(6, 5) for t in (tokens, g, h))
+    gen = torch.Generator(device="cuda").manual_seed(8)
+    res, branch, w, p, gate, dr, dy = (torch.randn(*s, generator=gen, device="cuda") for s in (
+        (2, 35, 96), (2, 35, 96), (96,), (96,), (2, 1, 96), (2, 35, 96), (2, 35, 96)))
+    leaves = [t.requires_grad_() for t in (res, branch, w, p, gate)]
+    return [
+        (lambda: (kernels.attention(q, k, v, lengths=lengths),), (q, k, v), (do,), 7),
+        (lambda: kernels.token_logprobs(x, tokens)[:2], (x,), (g, h), 4),
+        (lambda: kernels.residual_norm(*leaves[:3], post_weight=p, gate=gate), leaves, (dr, dy), 5),
+    ]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("which", range(3))
+def test_saved_tensors_laid_out_anew(which):
+    """Hooks that return one saved tensor, or all, in another layout: the same gradients."""
+    forward, leaves, given, saved = _steps_for_hooks()[which]
+    want = torch.autograd.grad(forward(), leaves, given)
+
+    def turned(t):
+        order = tuple(reversed(range(t.dim())))
+        return t.permute(order).contiguous().permute(order)
+
+    def shifted(t):  # dense, but at an address that is a multiple of no more than its element
+        return torch.cat((t.new_zeros(1), t.reshape(-1)))[1:].view(t.shape)
+
+    for change in (turned, shifted):
+        for one in (*range(saved), None):
+            count = 0
+
+            def pack(t):
+                nonlocal count
+                count += 1
+                return t.detach().clone(), count - 1
+
+            def unpack(packed):
+                t, i = packed
+                return change(t) if one is None or i == one else t
+
+            with torch.autograd.graph.saved_tensors_hooks(pack, unpack):
+                results = forward()
+            got = torch.autograd.grad(results, leaves, given)
+            assert count == saved
+            assert all(torch.equal(a, b) for a, b in zip(got, want)), (change.__name__, one)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("which", range(3))
+def test_saved_tensors_that_are_other_tensors(which):
+    """Hooks that return less than was saved, another type or another device: an error before any launch."""
+    forward, leaves, given, saved = _steps_for_hooks()[which]
+    for change in (lambda t: t[:1] if t.shape[0] > 1 else t[:0], lambda t: t.to(torch.float64), lambda t: t.cpu()):
+        for one in range(saved):
+            count = 0
+
+            def pack(t):
+                nonlocal count
+                count += 1
+                return t.detach().clone(), count - 1
+
+            with torch.autograd.graph.saved_tensors_hooks(pack, lambda p: change(p[0]) if p[1] == one else p[0]):
+                results = forward()
+            with pytest.raises(RuntimeError, match="came back from a hook|the model kernels have no"):
+                torch.autograd.grad(results, leaves, given)
+
+
 @pytest.mark.gpu
 def test_inputs_changed_before_the_backward_pass():
     """An error, not gradients of other inputs."""
