@@ -176,7 +176,9 @@ def token_logprobs(
         none = logits.sum(-1, dtype=torch.float32)  # empty, and still part of the graph
         ids = torch.empty((*tokens.shape, top), dtype=torch.int64, device=logits.device) if top else None
         return TokenLogprobs(none, none * 1, ids, None if ids is None else ids.float())
-    return TokenLogprobs(*_ops().token_logprobs(logits, tokens, top, ignore_index))
+    if top:
+        return TokenLogprobs(*_ops().token_logprobs_top(logits, tokens, top, ignore_index))
+    return TokenLogprobs(*_ops().token_logprobs(logits, tokens, ignore_index), None, None)
 
 
 # ------------------------------------------------------------------ residual norm
@@ -243,4 +245,6 @@ def residual_norm(
         for t in (branch, post_weight, gate):
             r = r if t is None else r * t.to(x.dtype)
         return (x if branch is None else r), (r * weight.to(x.dtype)).to(out_dtype)
+    if branch is None:
+        return x, _ops().rms_norm(x, weight, eps, out_dtype)
     return _ops().residual_norm(x, branch, weight, post_weight, gate, scale, eps, out_dtype)

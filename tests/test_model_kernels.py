@@ -156,6 +156,84 @@ def test_key_parts(ops, tokens):
         assert 1 <= ops.key_parts(1, 8, 2, tokens, 128, causal) <= 8
 
 
+def _meta_step(device="meta"):
+    """Arguments of every operator of the dispatcher's, in order, by name."""
+    def e(*shape, t=FP32):
+        return torch.empty(shape, dtype=t, device=device)
+
+    q, k, o, lse = e(2, 4, 9, 16, t=BF16), e(2, 2, 9, 16, t=BF16), e(2, 4, 9, 16, t=BF16), e(2, 4, 9)
+    lengths = e(2, t=torch.int32)
+    x, tokens, per, norm = e(2, 3, 50, t=BF16), e(2, 3, t=torch.int64), e(2, 3), e(6, 2)
+    r, b, w, gate = e(2, 3, 40), e(2, 3, 40, t=BF16), e(40), e(2, 1, 40)
+    return {
+        "attention": [q, k, k, lengths, 0.25, True],
+        "attention_forward": [q, k, k, lengths, 0.25, True],
+        "attention_backward": [o, q, k, k, o, o, lse, lengths, 0.25, True],
+        "token_logprobs": [x, tokens, -100],
+        "token_logprobs_top": [x, tokens, 5, -100],
+        "token_logprobs_forward": [x, tokens, 5, -100],
+        "token_logprobs_backward": [per, per, x, tokens, per, norm, -100],
+        "residual_norm": [r, b, w, w, gate, 1.0, 1e-5, BF16],
+        "rms_norm": [r, w, 1e-5, BF16],
+        "residual_norm_backward": [r, b, r, b, w, w, gate, 1.0, 1e-5, BF16, BF16, 31],
+    }
+
+
+def test_dispatched_operators_check_what_they_are_given(ops):
+    """Called past workloads.kernels, each refuses a tensor that is smaller, of another type or of another rank."""
+    for name, args in _meta_step().items():
+        f = getattr(torch.ops.sofa_model, name)
+        f(*args)
+        for i, t in enumerate(args):
+            if not isinstance(t, torch.Tensor):
+                continue
+            for wrong in (t[..., 1:], t[1:], t.to(torch.float64), t[None], t[..., :0]):
+                if wrong.numel() and wrong.dtype == t.dtype and (
+                        name == "rms_norm" and i == 0 and wrong.shape[-1] == 40  # other rows
+                        or name.startswith("token_logprobs") and wrong.shape == (2, 3, 49)):  # another vocabulary
+                    continue
+                with pytest.raises(RuntimeError, match="does not belong|the model kernels have no"):
+                    f(*args[:i], wrong, *args[i + 1:])
+    for wrong in (-1, 33, 51):
+        with pytest.raises(RuntimeError, match="does not belong|no alternatives"):
+            torch.ops.sofa_model.token_logprobs_top(*_meta_step()["token_logprobs_top"][:2], wrong, -100)
+    for bits, post, gate in ((8, None, True), (16, True, None)):
+        args = _meta_step()["residual_norm_backward"]
+        args[5], args[6], args[-1] = post and args[5], gate and args[6], bits
+        with pytest.raises(RuntimeError, match="what is not there"):
+            torch.ops.sofa_model.residual_norm_backward(*args)
+
+
+def test_fake_tensors_and_make_fx(ops):
+    """Shapes, types and layouts without data, and each operator as a node of a recorded graph."""
+    from torch._subclasses.fake_tensor import FakeTensorMode
+    from torch.fx.experimental.proxy_tensor import make_fx
+
+    def step(q, k, v, x, tokens, res, branch, w):
+        o = kernels.attention(q, k, v)
+        r, y = kernels.residual_norm(res, branch, w, post_weight=w, out_dtype=BF16)
+        z = kernels.residual_norm(r, None, w)[1]
+        return o, r, y, z, *kernels.token_logprobs(x, tokens, top=3), kernels.token_logprobs(x, tokens).logprob
+
+    with FakeTensorMode():
+        def e(*shape, t=FP32):
+            return torch.empty(shape, dtype=t, device="cuda")
+
+        args = [e(2, 9, 4, 16, t=BF16).transpose(1, 2), *(e(2, 9, 2, 16, t=BF16).transpose(1, 2) for _ in range(2)),
+                e(2, 3, 50, t=BF16), e(2, 3, t=torch.int64), e(2, 3, 40), e(2, 3, 40, t=BF16), e(40)]
+        for grad in (False, True):
+            o, r, y, z, logprob, entropy, ids, values, again = step(*(t.requires_grad_(grad and t.is_floating_point()) for t in args))
+            assert o.shape == (2, 4, 9, 16) and o.dtype == BF16 and o.transpose(1, 2).is_contiguous()
+            assert r.shape == y.shape == z.shape == (2, 3, 40) and (r.dtype, y.dtype, z.dtype) == (FP32, BF16, FP32)
+            assert logprob.shape == entropy.shape == again.shape == (2, 3) and logprob.dtype == FP32
+            assert ids.shape == values.shape == (2, 3, 3) and (ids.dtype, values.dtype) == (torch.int64, FP32)
+            assert all(t.device.type == "cuda" and t.requires_grad == grad for t in (o, r, y, z, logprob, entropy, again))
+        graph = make_fx(step)(*(t.detach() for t in args)).graph
+    called = [n.target.name() for n in graph.nodes if n.op == "call_function" and str(n.target).startswith("sofa_model")]
+    assert called == ["sofa_model::attention", "sofa_model::residual_norm", "sofa_model::rms_norm",
+                      "sofa_model::token_logprobs_top", "sofa_model::token_logprobs"]
+
+
 # ------------------------------------------------------------------ attention
 def attention_64(q, k, v, do, lengths, causal, scale):
     """Results, gradients and their bounds by the formulas, in 64 bits, one head at a time."""
@@ -912,6 +990,71 @@ def test_first_derivatives_only():
             first.sum().backward()
 
 
+def _traced_functions():
+    lengths = torch.tensor([150, 40], dtype=torch.int32, device="cuda")
+    return [
+        (lambda q, k, v: kernels.attention(q, k, v, lengths=lengths), lambda s: s[:3]),
+        (lambda x, ids: tuple(kernels.token_logprobs(x, ids, top=3)), lambda s: (s[4], s[5])),
+        (lambda x, ids: kernels.token_logprobs(x, ids)[:2], lambda s: (s[4], s[5])),
+        (lambda r, w: kernels.residual_norm(r, r.neg(), w, post_weight=w, scale=0.5), lambda s: s[8:]),
+        (lambda r, w: kernels.residual_norm(r, None, w)[1], lambda s: s[8:]),
+    ]
+
+
+@pytest.mark.gpu
+@pytest.mark.filterwarnings("ignore::torch.jit.TracerWarning", "ignore::DeprecationWarning")
+@pytest.mark.parametrize("which", range(5))
+def test_traced(which):
+    """Recorded by torch's tracers and run on other inputs: the same results and gradients."""
+    from torch.fx.experimental.proxy_tensor import make_fx
+
+    f, pick = _traced_functions()[which]
+
+    def flat(out):
+        return list(out) if isinstance(out, tuple) else [out]
+
+    def inputs(seed, grad):
+        return [t.requires_grad_(grad and t.is_floating_point()) for t in pick(_step(seed))]
+
+    def grads(out, leaves):
+        outs = [t for t in flat(out) if t.requires_grad]
+        leaves = [t for t in leaves if t.requires_grad]
+        return torch.autograd.grad(outs, leaves, [torch.full_like(t, 0.5) for t in outs]) if outs else ()
+
+    for grad in (False, True):
+        traced = torch.jit.trace(f, inputs(11, grad))
+        for seed in (12, 13):
+            got_in, want_in = inputs(seed, grad), inputs(seed, grad)
+            got, want = traced(*got_in), f(*want_in)
+            for a, b in zip((*flat(got), *grads(got, got_in)), (*flat(want), *grads(want, want_in))):
+                assert torch.equal(a, b) and a.requires_grad == b.requires_grad
+
+    def step(*args):  # with its backward pass
+        leaves = [t.detach().requires_grad_() if t.is_floating_point() else t for t in args]
+        out = f(*leaves)
+        return (*(t.detach() for t in flat(out)), *grads(out, leaves))
+
+    graph = make_fx(step)(*inputs(11, False))
+    for seed in (12, 13):
+        for a, b in zip(graph(*inputs(seed, False)), step(*inputs(seed, False))):
+            assert torch.equal(a, b)
+
+
+@pytest.mark.gpu
+@pytest.mark.filterwarnings("ignore::UserWarning")  # torch warns that it maps over the calls one by one
+def test_mapped_over_a_batch():
+    """torch.func: vmap is each call by itself; its gradient transforms do not know C++ functions and say so."""
+    q, k, v = (x.detach() for x in attention_case(2, 4, 2, 40, 64, seed=6)[:3])
+    stacked = [torch.stack((x, x.flip(2), x * 0.5)) for x in (q, k, v)]
+    got = torch.vmap(kernels.attention)(*stacked)
+    assert all(torch.equal(got[i], kernels.attention(*(x[i] for x in stacked))) for i in range(3))
+    r, w = torch.randn(3, 5, 64, device="cuda"), torch.ones(64, device="cuda")
+    got = torch.vmap(lambda x: kernels.residual_norm(x, x, w)[1])(r)
+    assert torch.equal(got, kernels.residual_norm(r, r, w)[1])
+    with pytest.raises(RuntimeError):
+        torch.func.grad(lambda x: kernels.residual_norm(x, x, w)[1].sum())(r)
+
+
 @pytest.mark.gpu
 def test_recomputed_and_offloaded():
     """What a backward pass needs may be computed again or come back from host memory, laid out anew."""
@@ -1007,7 +1150,7 @@ def test_saved_tensors_that_are_other_tensors(which):
 
             with torch.autograd.graph.saved_tensors_hooks(pack, lambda p: change(p[0]) if p[1] == one else p[0]):
                 results = forward()
-            with pytest.raises(RuntimeError, match="came back from a hook|the model kernels have no"):
+            with pytest.raises(RuntimeError, match="does not belong to the other tensors|the model kernels have no"):
                 torch.autograd.grad(results, leaves, given)
 
 
