@@ -95,8 +95,13 @@ const auto& op(const char* name) {
   return handle;
 }
 
-// Whether autograd will ask for a backward pass
+// Whether autograd will ask for a backward pass. Derivatives that are carried
+// forward are refused here: a result without one would read as not depending on
+// the input.
 bool recorded(std::initializer_list<Tensor> tensors) {
+  for (const Tensor& t : tensors)
+    TORCH_CHECK(!t.defined() || !t._fw_grad(0).defined(),
+                "the model kernels have no forward-mode derivatives");
   if (!at::GradMode::is_enabled()) return false;
   for (const Tensor& t : tensors)
     if (t.defined() && t.requires_grad()) return true;

@@ -4,7 +4,7 @@
     token_logprobs(logits, ids)   log p(token), entropy, alternatives
     residual_norm(x, branch, w)   residual sum and the RMS norm of it
 
-All three are differentiable (first derivatives), run on the current stream of
+All three are differentiable (first derivatives, backward mode), run on the current stream of
 their tensors' device, allocate what they return and nothing that outlives the
 call, give the same bits for the same inputs, and can be captured into a graph
 (a backward pass, as always with torch, while no eager graph of its leaves lives).

@@ -990,6 +990,29 @@ def test_first_derivatives_only():
             first.sum().backward()
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("grad", [False, True])
+def test_forward_mode_is_refused(grad):
+    """A tangent on any differentiable argument is an error, not a result without one."""
+    import torch.autograd.forward_ad as fw
+
+    q, k, v, x, tokens, res, w = (_step()[i] for i in (0, 1, 2, 4, 5, 8, 9))
+    gate = torch.ones(2, 1, 256, device="cuda")
+    for f, args in (
+        (kernels.attention, [q, k, v]),
+        (lambda x: kernels.token_logprobs(x, tokens), [x]),
+        (lambda x: kernels.token_logprobs(x, tokens, top=2), [x]),
+        (lambda x, w: kernels.residual_norm(x, None, w), [res, w]),
+        (lambda x, b, w, p, g: kernels.residual_norm(x, b, w, post_weight=p, gate=g), [res, res.clone(), w, w.clone(), gate]),
+    ):
+        for i, t in enumerate(args):
+            with fw.dual_level(), torch.set_grad_enabled(grad):
+                dual = fw.make_dual(t.detach(), torch.ones_like(t))
+                with pytest.raises(RuntimeError, match="forward-mode"):
+                    f(*args[:i], dual, *args[i + 1:])
+        f(*args)
+
+
 def _traced_functions():
     lengths = torch.tensor([150, 40], dtype=torch.int32, device="cuda")
     return [
