@@ -670,6 +670,8 @@ attention_dkv_kernel(AttentionArgs a) {
       s[i / 16][i % 16] = p;
       dp[i / 16][i % 16] *= p;
     }
+    // row 0 sees key 0 alone: dS is 0, not what roundings leave of dP - delta
+    if (MASKED && first == 0 && h == 0) dp[0][0] = 0.f;
 #pragma unroll
     for (int p = 0; p < 2 * kBlocks; ++p) {
       const bf16x8 probs = rounded(s[p / 2], p % 2);

@@ -351,6 +351,17 @@ def test_attention_one_key(t, d, lengths, causal):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("t, d, lengths", [(40, 16, None), (64, 64, [64, 30]), (300, 128, None), (700, 40, [700, 2])])
+def test_attention_first_key_of_the_first_token(t, d, lengths):
+    """Under a causal mask the first token sees its own key alone and passes nothing on to that either."""
+    q, k, v, do = attention_case(2, 4, 2, t, d, seed=23, std=3.0)
+    do[:, :, 1:] = 0
+    valid = None if lengths is None else torch.tensor(lengths, dtype=torch.int32, device="cuda")
+    dq, dk, _ = torch.autograd.grad(kernels.attention(q, k, v, lengths=valid), (q, k, v), do)
+    assert not dq.any() and not dk.any()
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("causal", [True, False])
 @pytest.mark.parametrize("h, kv, t, d", [(2, 1, 1100, 24), (2, 2, 600, 8), (1, 1, 257, 32), (3, 3, 256, 16)])
 def test_attention_short_heads(h, kv, t, d, causal):
