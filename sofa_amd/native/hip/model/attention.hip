@@ -285,7 +285,8 @@ __device__ __forceinline__ int valid_tokens(const AttentionArgs& a, int batch) {
 // Short heads of long rows: four workgroups on a compute unit, at the cost of a
 // register spilled (2 x 4096 tokens, 32/8 heads of 64, no mask: 325 us in place of
 // 340 with three); a few hundred tokens do not fill them, and lose 3 %.
-template <int DP, bool CAUSAL, bool SHORT>
+// KEEP: with lse, whose own sum of the probabilities takes 4 % of the time.
+template <int DP, bool CAUSAL, bool SHORT, bool KEEP>
 __global__ __launch_bounds__(kThreads, DP > 64 ? 2 : SHORT ? 3 : 4)
 void attention_forward_kernel(
     AttentionArgs a) {
@@ -313,8 +314,8 @@ void attention_forward_kernel(
   // l sums what 16 bits leave of the probabilities, since it divides their
   // product: the weights are 1 together then. (Summed before they are rounded, a
   // row with one large probability is off by all of its rounding, and dP - delta,
-  // almost 0 there, by more than itself.) lse takes the same l, 2^-8 off at most;
-  // SHORT: their sum before they are rounded.
+  // almost 0 there, by more than itself.) lse takes their sum before they are
+  // rounded: what the backward pass computes from it is not rounded yet.
   float m = -INFINITY, l = 0.f, l_exact = 0.f;
   const float scale = a.scale * kLog2e;
 
@@ -355,14 +356,14 @@ void attention_forward_kernel(
       const float fade = exp2_fast(m - next);
       m = next;
       l *= fade;
-      if (SHORT) l_exact *= fade;
+      if (KEEP) l_exact *= fade;
 #pragma unroll
       for (int b = 0; b < DP / 32; ++b) acc[b] *= fade;
     }
 #pragma unroll
     for (int i = 0; i < 32; ++i) {
       const float p = exp2_fast(s[i / 16][i % 16] * scale - m);
-      if (SHORT) l_exact += p;
+      if (KEEP) l_exact += p;
       s[i / 16][i % 16] = p;
     }
 #pragma unroll
@@ -391,9 +392,9 @@ void attention_forward_kernel(
   }
 
   l += other_half(l);
-  l_exact = SHORT ? l_exact + other_half(l_exact) : l;
+  if (KEEP) l_exact += other_half(l_exact);
   const bool valid = row < n;
-  if (row < a.tokens && a.lse && h == 0)
+  if (KEEP && row < a.tokens && h == 0)
     a.lse[(int64_t) bh * a.tokens + row] =
         valid ? m + log2_fast(l_exact) : INFINITY;
   __syncthreads();  // the tiles are not read any more
@@ -759,19 +760,25 @@ __global__ __launch_bounds__(kThreads) void attention_join_kernel(
          sum);
 }
 
-template <int DP, bool CAUSAL, bool SHORT>
+template <int DP, bool CAUSAL, bool SHORT, bool KEEP>
 int forward(const AttentionArgs& a) {
   const int64_t blocks = (a.tokens + kRows - 1) / kRows;
-  hipLaunchKernelGGL((attention_forward_kernel<DP, CAUSAL, SHORT>),
+  hipLaunchKernelGGL((attention_forward_kernel<DP, CAUSAL, SHORT, KEEP>),
                      dim3((unsigned) (blocks * a.batch * a.heads)),
                      dim3(kThreads), 0, static_cast<hipStream_t>(a.stream), a);
   return (int) hipGetLastError();
 }
 
-template <int DP, bool CAUSAL>
+template <int DP, bool CAUSAL, bool KEEP>
 int forward(const AttentionArgs& a) {
-  return a.tokens <= kShort ? forward<DP, CAUSAL, true>(a)
-                            : forward<DP, CAUSAL, false>(a);
+  return DP <= 64 && a.tokens <= kShort ? forward<DP, CAUSAL, DP <= 64, KEEP>(a)
+                                        : forward<DP, CAUSAL, false, KEEP>(a);
+}
+
+template <int DP>
+int forward(const AttentionArgs& a) {
+  if (a.lse) return a.causal ? forward<DP, true, true>(a) : forward<DP, false, true>(a);
+  return a.causal ? forward<DP, true, false>(a) : forward<DP, false, false>(a);
 }
 
 template <int DP, bool CAUSAL, bool SHORT>
@@ -835,9 +842,7 @@ int sofa_attention_forward(const sofa_model::AttentionArgs* a) {
   if (!sound(a)) return kBadArgument;
   DeviceGuard guard(a->device);
   if (guard.status()) return guard.status();
-  if (a->dim <= 64)
-    return a->causal ? forward<64, true>(*a) : forward<64, false>(*a);
-  return a->causal ? forward<128, true>(*a) : forward<128, false>(*a);
+  return a->dim <= 64 ? forward<64>(*a) : forward<128>(*a);
 }
 
 int sofa_attention_backward(const sofa_model::AttentionArgs* a) {

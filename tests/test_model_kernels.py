@@ -396,6 +396,34 @@ def test_attention_short_rows_take_more_of_p(h, kv, t, d, causal):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("d", [16, 64, 128])
+def test_attention_normalizes_by_what_is_not_rounded(d):
+    """Probabilities that all round the same way: their sum as they are is what the backward pass divides by."""
+    # Scores in units of log 2, the same in every row. Six keys, the first, have e^(S - max) of four times 1, 2^-6 and
+    # 2^-10, 4.0166... together, and 1016 have p = 4.0166.../8, just above the middle of two bf16 numbers. The sum is 1024 p
+    # and P = 2^-10, which bf16 holds; the sum of the rounded p is 0.36 % larger, and P over that rounds to the
+    # number below.
+    many, few = 1016, torch.tensor([0.0, 0.0, 0.0, 0.0, -6.0, -10.0], device="cuda", dtype=torch.float64)
+    p = torch.exp2(few).sum() / 8
+    assert p.to(BF16) / p > 1 + 0.9 * U[BF16]
+    rest = torch.log2(p)
+    t = many + len(few)
+    k = torch.zeros(1, 1, t, d, dtype=BF16, device="cuda")
+    k[0, 0, :6, 0] = few.to(BF16)
+    for i in range(3):  # 24 bits of it, 8 at a time
+        k[0, 0, 6:, i] = rest.to(BF16)
+        rest = rest - rest.to(BF16).double()
+    q = torch.zeros(1, 1, t, d, dtype=BF16, device="cuda")
+    q[..., :3] = 1
+    v = torch.randn(1, 1, t, d, device="cuda").to(BF16).requires_grad_()
+    do = torch.zeros_like(q)
+    do[:, :, :512] = 1
+    (dv,) = torch.autograd.grad(kernels.attention(q, k, v, causal=False, scale=math.log(2)), v, do)
+    # 512 times 2^-10: every step is exact
+    assert (dv[:, :, 6:] == 0.5).all()
+
+
+@pytest.mark.gpu
 def test_attention_large_scores():
     """Scores in the hundreds: a softmax that is almost a choice; a scale of the caller's."""
     check_attention(*attention_case(1, 2, 1, 200, 64, std=8.0), scale=0.2)
