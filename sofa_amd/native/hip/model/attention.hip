@@ -1,12 +1,16 @@
 // Self-attention over grouped heads and its gradients, on the matrix cores.
 //
-//   S = c Q K^T + mask      P = softmax(S) = e^(S - lse)       O = P V
+//   S = c Q K^T + mask      P = softmax(S) = e^(S - lse) = e^(c (Q K^T - L))
+//   O = P V
 //   dV = P^T dO             dP = dO V^T       delta = rowsum(dO O)
 //   dS = P (dP - delta)     dQ = c dS K       dK = c dS^T Q
 //
 // The scores are never stored: the forward pass runs over the keys with a
-// running maximum and sum (in 32 bits, base 2) and keeps lse; the backward
-// pass computes P again from it.  It is two kernels, one that owns rows of
+// running maximum and sum (in 32 bits, base 2) and keeps L = lse / c, in units
+// of the products: a row that is sure of one key has L equal to that product, bit
+// by bit, however large it is, and the backward pass computes P = 1 again.  (lse
+// itself, next to scores in the hundred thousands, is 2^-6 apart.)  The products
+// are summed in the same order each time.  The backward pass is two kernels, one that owns rows of
 // dQ and one that owns rows of dK and dV (over all heads that share them):
 // 7 products in place of 5, but no atomics, so the same bits every time.
 //
@@ -317,6 +321,7 @@ void attention_forward_kernel(
   // almost 0 there, by more than itself.) lse takes their sum before they are
   // rounded: what the backward pass computes from it is not rounded yet.
   float m = -INFINITY, l = 0.f, l_exact = 0.f;
+  float largest = -INFINITY;  // KEEP: of the products
   const float scale = a.scale * kLog2e;
 
   int end = block * kRows < n ? n : 0;
@@ -348,6 +353,7 @@ void attention_forward_kernel(
 #pragma unroll
     for (int i = 1; i < 32; ++i) most = fmaxf(most, s[i / 16][i % 16]);
     most = fmaxf(most, other_half(most));
+    if (KEEP) largest = fmaxf(largest, most);
     // m follows the maximum in steps of 2^8 or more: the probabilities are
     // relative to it anyway, and most tiles need no new factor for the sums.
     // The first tile holds key 0, which every row sees: m is finite after it.
@@ -362,7 +368,7 @@ void attention_forward_kernel(
     }
 #pragma unroll
     for (int i = 0; i < 32; ++i) {
-      const float p = exp2_fast(s[i / 16][i % 16] * scale - m);
+      const float p = exp2_fast(fmaf(s[i / 16][i % 16], scale, -m));
       if (KEEP) l_exact += p;
       s[i / 16][i % 16] = p;
     }
@@ -396,7 +402,10 @@ void attention_forward_kernel(
   const bool valid = row < n;
   if (KEEP && row < a.tokens && h == 0)
     a.lse[(int64_t) bh * a.tokens + row] =
-        valid ? m + log2_fast(l_exact) : INFINITY;
+        // m is the rounding of a product's multiple, or lags behind: what the sum
+        // is relative to, less that
+        valid ? largest + (log2_fast(l_exact) - fmaf(largest, scale, -m)) / scale
+              : INFINITY;
   __syncthreads();  // the tiles are not read any more
   bf16* stage = k_tiles[0] + wave * 32 * DP;
   const int64_t o_at = batch * a.o_stride[0] + head * a.o_stride[1] +
@@ -462,10 +471,13 @@ void attention_dq_kernel(
   if (row < a.tokens && h == 0) a.delta[at] = delta;
   // +inf makes every probability of a row without keys 0; and with one key alone
   // dS is 0, not what roundings leave of dP - delta
-  const bool alone = n == 1 || (CAUSAL && row == 0);
-  const float lse = valid && !alone ? a.lse[at] : INFINITY;
-  floatx16 acc[DP / 32] = {};
+  const bool sees = valid && !(n == 1 || (CAUSAL && row == 0));
   const float scale = a.scale * kLog2e;
+  const float start = sees ? a.lse[at] : 0.f;
+  const float lse = sees ? start * scale : INFINITY;
+  // what that product's rounding took off is a factor of the whole row
+  const float factor = a.scale * (sees ? exp2_fast(-fmaf(start, scale, -lse)) : 1.f);
+  floatx16 acc[DP / 32] = {};
 
   int end = block * kRows < n ? n : 0;
   if (CAUSAL) end = min(end, (block + 1) * kRows);
@@ -496,7 +508,7 @@ void attention_dq_kernel(
       if (part == 2 / kBlocks - 1) load(first + kTile, buffer ^ 1);
 #pragma unroll
       for (int i = 0; i < 16 * kBlocks; ++i) {
-        float p = exp2_fast(s[i / 16][i % 16] * scale - lse);
+        float p = exp2_fast(fmaf(s[i / 16][i % 16], scale, -lse));
         if (MASKED) {
           const int key = first + line + i / 4 * 8 + h * 4 + i % 4;
           if (key >= n || (CAUSAL && key > row)) p = 0.f;
@@ -534,7 +546,7 @@ void attention_dq_kernel(
   store_rows<DP>(k_tiles[0] + wave * 32 * DP,
                  a.dq + batch * a.dq_stride[0] + head * a.dq_stride[1] +
                      (int64_t) wave_row * a.dq_stride[2],
-                 a.dq_stride[2], a.tokens - wave_row, a.dim, acc, a.scale,
+                 a.dq_stride[2], a.tokens - wave_row, a.dim, acc, factor,
                  valid);
 }
 
@@ -557,8 +569,7 @@ attention_dkv_kernel(AttentionArgs a) {
   __shared__ __align__(16) bf16 tiles_of[2][2][kLines * DP];
   bf16(*q_tiles)[kLines * DP] = tiles_of[0];
   bf16(*do_tiles)[kLines * DP] = tiles_of[1];
-  // what the products of a row start from: -lse in units of the scores, and
-  // -delta
+  // lse, and -delta, which the products of a row start from
   __shared__ __align__(16) float lse_tiles[2][kLines];
   __shared__ __align__(16) float delta_tiles[2][kLines];
   const int blocks = (a.tokens + kRows - 1) / kRows;
@@ -628,28 +639,21 @@ attention_dkv_kernel(AttentionArgs a) {
       delta = a.delta[at];
     }
   };
-  const float inv_scale = 1.f / scale;
   auto store = [&](int buffer) {
     if (threadIdx.x < kLines) {
-      lse_tiles[buffer][threadIdx.x] = -lse * inv_scale;
+      lse_tiles[buffer][threadIdx.x] = lse;
       delta_tiles[buffer][threadIdx.x] = -delta;
     }
   };
   auto tile = [&]<bool MASKED>(int step, int buffer) {
     const bf16 *q_tile = q_tiles[buffer], *do_tile = do_tiles[buffer];
-    floatx16 s[kBlocks], dp[kBlocks];
+    floatx16 s[kBlocks] = {}, dp[kBlocks];
 #pragma unroll
     for (int i = 0; i < 4 * kBlocks; ++i) {
-      const int line = i * 8 + h * 4;
-      const floatx4 x =
-          *reinterpret_cast<const floatx4*>(lse_tiles[buffer] + line);
       const floatx4 y =
-          *reinterpret_cast<const floatx4*>(delta_tiles[buffer] + line);
+          *reinterpret_cast<const floatx4*>(delta_tiles[buffer] + i * 8 + h * 4);
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        s[i / 4][i % 4 * 4 + j] = x[j];
-        dp[i / 4][i % 4 * 4 + j] = y[j];
-      }
+      for (int j = 0; j < 4; ++j) dp[i / 4][i % 4 * 4 + j] = y[j];
     }
 #pragma unroll
     for (int d = 0; d < DP / 16; ++d)
@@ -665,11 +669,18 @@ attention_dkv_kernel(AttentionArgs a) {
     load(step + 1, buffer ^ 1);
     const int first = start + (tiles - 1 - step % tiles) * kLines;
 #pragma unroll
-    for (int i = 0; i < 16 * kBlocks; ++i) {
-      float p = exp2_fast(s[i / 16][i % 16] * scale);
-      if (MASKED && key > first + i / 4 * 8 + h * 4 + i % 4) p = 0.f;
-      s[i / 16][i % 16] = p;
-      dp[i / 16][i % 16] *= p;
+    for (int i = 0; i < 4 * kBlocks; ++i) {
+      const int line = i * 8 + h * 4;
+      const floatx4 x =
+          *reinterpret_cast<const floatx4*>(lse_tiles[buffer] + line);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const int at = i % 4 * 4 + j;
+        float p = exp2_fast((s[i / 4][at] - x[j]) * scale);
+        if (MASKED && key > first + line + j) p = 0.f;
+        s[i / 4][at] = p;
+        dp[i / 4][at] *= p;
+      }
     }
     // row 0 sees key 0 alone: dS is 0, not what roundings leave of dP - delta
     if (MASKED && first == 0 && h == 0) dp[0][0] = 0.f;

@@ -35,7 +35,7 @@ struct AttentionArgs {
   const bf16 *q, *k, *v;  // [batch][heads][tokens][dim] by strides, dim dense
   bf16* o;
   bf16* o_low;            // what rounding took off o, laid out like it; or null
-  float* lse;             // [batch][heads][tokens], base 2; +inf: no keys
+  float* lse;             // [batch][heads][tokens], over scale; +inf: no keys
   const int* lengths;     // [batch] valid tokens, or null
   const bf16* dout;
   float* delta;           // [batch][heads][tokens]

@@ -430,6 +430,31 @@ def test_attention_large_scores():
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("causal", [True, False])
+@pytest.mark.parametrize("t, d", [(90, 64), (250, 128), (700, 128), (700, 64), (600, 24)])
+def test_attention_scores_in_the_hundred_thousands(t, d, causal):
+    """Each token chooses one key outright: its probability is 1 in the backward pass too."""
+    g = torch.Generator(device="cuda").manual_seed(t + d)
+    q, k, v, do = (torch.randn(1, 2, t, d, generator=g, device="cuda").mul(std).to(BF16) for std in (300.0, 300.0, 1.0, 1.0))
+    s = 0.25 * q.double() @ k.double().transpose(-1, -2)
+    if causal:
+        s = s.masked_fill(torch.ones(t, t, dtype=torch.bool, device="cuda").triu(1), -math.inf)
+    best = s.topk(2, -1)
+    assert best.values[..., 0].median() > 1e5
+    # scores are off by 2^-24 of up to d additions of products of 1e6: with 200 between them, and e^-200 below 2^-126,
+    # P is 1 and 0. The rows of closer choices pass nothing on.
+    sure = best.values[..., :1] - best.values[..., 1:] > 200
+    assert sure.double().mean() > 0.9
+    do = do * sure
+    v.requires_grad_()
+    (dv,) = torch.autograd.grad(kernels.attention(q, k, v, causal=causal, scale=0.25), v, do)
+    at = best.indices[..., :1].expand(do.shape)
+    want = torch.zeros(do.shape, dtype=torch.float64, device="cuda").scatter_add_(2, at, do.double())
+    size = torch.zeros_like(want).scatter_add_(2, at, do.double().abs())
+    close(dv, want, U[BF16] * want.abs() + t * STEP * size, "dv")
+
+
+@pytest.mark.gpu
 def test_attention_strides():
     """Heads first, an expanded key head, rows that are not dense, rows at odd places."""
     q, k, v, do = (x.detach() for x in attention_case(2, 4, 2, 90, 64, seed=3))
