@@ -57,7 +57,8 @@ constexpr int kThreads = 256;
 constexpr int kWaves = 4;
 constexpr int kRows = kWaves * 32;  // rows a workgroup owns
 constexpr int kTile = 64;           // rows of the other side at a time
-constexpr int kShort = 256;         // tokens up to which P and dS have 16 bits
+constexpr int kShort = 256;         // tokens that leave a compute unit room
+constexpr int kFewKeys = 256;       // up to which P and dS have 16 bits
 
 // Where the 8 elements `chunk` of `row` of a tile are in LDS.  A row is 256 or
 // 128 bytes and the banks 256, so one chunk of all rows falls on the same banks;
@@ -419,12 +420,14 @@ void attention_forward_kernel(
 
 // dQ, and delta for the other kernel.
 //
-// SHORT: dS, and P for dV, are taken with 16 bits, as their rounding and what
-// that took off.  In long rows their rounding is one of many and leaves the
-// gradients 1.4 times as far off as their own rounding does; in short ones it
-// was up to 1.8 times.  There the products that this adds are not what takes
-// the time.
-template <int DP, bool CAUSAL, bool SHORT>
+// EXACT, and for rows that see up to kFewKeys keys: dS, and P for dV, are taken
+// with 16 bits, as their rounding and what that took off.  In long rows their
+// rounding is one of many and leaves the gradients 1.4 times as far off as their
+// own rounding does; in short ones it was up to 1.8 times.  The rule is one of the
+// keys that a workgroup's rows see, so that a sequence is as exact in whatever
+// batch, and the first rows of a long one as a short one.  The
+// products that this adds are not what takes the time there.
+template <int DP, bool CAUSAL, bool EXACT>
 __global__ __launch_bounds__(kThreads, DP > 64 ? 2 : 3)
 void attention_dq_kernel(
     AttentionArgs a) {
@@ -491,7 +494,7 @@ void attention_dq_kernel(
   // 32 kBlocks keys at a time: short heads gain more from a third workgroup on
   // the compute unit (168 registers) than from two independent chains
   constexpr int kBlocks = DP <= 64 ? 1 : 2;
-  auto tile = [&]<bool MASKED>(int first, int buffer) {
+  auto tile = [&]<bool MASKED, bool FEW>(int first, int buffer) {
     const bf16 *k_tile = k_tiles[buffer], *v_tile = v_tiles[buffer];
 #pragma unroll
     for (int part = 0; part < 2 / kBlocks; ++part) {
@@ -522,26 +525,32 @@ void attention_dq_kernel(
         for (int c = 0; c < DP / 32; ++c) {
           const bf16x8 keys = column_operand<DP>(k_tile, line + p * 16, c);
           acc[c] = mfma(keys, ds, acc[c]);
-          if (SHORT) acc[c] = mfma(keys, rest_of(s[p / 2], p % 2, ds), acc[c]);
+          if (FEW) acc[c] = mfma(keys, rest_of(s[p / 2], p % 2, ds), acc[c]);
         }
       }
     }
   };
   // tiles that every row sees whole, then the others
   const int whole = (CAUSAL ? min(block * kRows, n) : n) / kTile * kTile;
-  int first = 0, buffer = 0;
-  load(0, 0);
-  for (; first < min(whole, end); first += kTile, buffer ^= 1) {
-    arrived();
-    tile.template operator()<false>(first, buffer);
-  }
-  for (; first < end; first += kTile, buffer ^= 1) {
-    arrived();
-    if (CAUSAL && first > wave_row + 31)
-      load(first + kTile, buffer ^ 1);
-    else
-      tile.template operator()<true>(first, buffer);
-  }
+  auto all = [&]<bool FEW>() {
+    int first = 0, buffer = 0;
+    load(0, 0);
+    for (; first < min(whole, end); first += kTile, buffer ^= 1) {
+      arrived();
+      tile.template operator()<false, FEW>(first, buffer);
+    }
+    for (; first < end; first += kTile, buffer ^= 1) {
+      arrived();
+      if (CAUSAL && first > wave_row + 31)
+        load(first + kTile, buffer ^ 1);
+      else
+        tile.template operator()<true, FEW>(first, buffer);
+    }
+  };
+  if (EXACT || end <= kFewKeys)
+    all.template operator()<true>();
+  else
+    all.template operator()<false>();
   __syncthreads();  // the tiles are not read any more
   store_rows<DP>(k_tiles[0] + wave * 32 * DP,
                  a.dq + batch * a.dq_stride[0] + head * a.dq_stride[1] +
@@ -559,6 +568,13 @@ void attention_dq_kernel(
 // is in LDS then and tiles have 32 rows.  With V in registers too and one
 // workgroup (of 64 rows a tile) the same 2 x 4096 tokens, 32/8 heads, took 1.26
 // ms in place of 1.04, without a mask.
+//
+// P and dS of rows that see up to kFewKeys keys have 16 bits, as in dQ.  SHORT: all
+// of them, next to the products of what rounding leaves.  Otherwise the tiles of
+// such rows are gone over once more for the products of the rest: in the loop
+// over all tiles a second body, or a branch, takes 9 to 30 % (registers).  Those of
+// longer rows have one rounding each for heads of up to 32 too, where dQ has 16
+// bits: it would take 121 us in place of 80 at 2 x 2048 tokens, 32 heads of 16.
 template <int DP, bool CAUSAL, bool SHORT>
 __global__ __launch_bounds__(kThreads, 2) void
 attention_dkv_kernel(AttentionArgs a) {
@@ -645,7 +661,8 @@ attention_dkv_kernel(AttentionArgs a) {
       delta_tiles[buffer][threadIdx.x] = -delta;
     }
   };
-  auto tile = [&]<bool MASKED>(int step, int buffer) {
+  // REST: the products of what rounding takes off P and dS; `next` comes after it
+  auto tile = [&]<bool MASKED, bool REST>(int step, int next, int buffer) {
     const bf16 *q_tile = q_tiles[buffer], *do_tile = do_tiles[buffer];
     floatx16 s[kBlocks] = {}, dp[kBlocks];
 #pragma unroll
@@ -666,7 +683,7 @@ attention_dkv_kernel(AttentionArgs a) {
           dp[b] = mfma(row_operand<DP>(do_tile, b * 32, d),
                        row_operand<DP>(v_rows, wave * 32, d), dp[b]);
       }
-    load(step + 1, buffer ^ 1);
+    load(next, buffer ^ 1);
     const int first = start + (tiles - 1 - step % tiles) * kLines;
 #pragma unroll
     for (int i = 0; i < 4 * kBlocks; ++i) {
@@ -686,8 +703,12 @@ attention_dkv_kernel(AttentionArgs a) {
     if (MASKED && first == 0 && h == 0) dp[0][0] = 0.f;
 #pragma unroll
     for (int p = 0; p < 2 * kBlocks; ++p) {
-      const bf16x8 probs = rounded(s[p / 2], p % 2);
-      const bf16x8 ds = rounded(dp[p / 2], p % 2);
+      bf16x8 probs = rounded(s[p / 2], p % 2);
+      bf16x8 ds = rounded(dp[p / 2], p % 2);
+      if (REST) {
+        probs = rest_of(s[p / 2], p % 2, probs);
+        ds = rest_of(dp[p / 2], p % 2, ds);
+      }
 #pragma unroll
       for (int c = 0; c < DP / 32; ++c) {
         const bf16x8 douts = column_operand<DP>(do_tile, p * 16, c);
@@ -700,6 +721,7 @@ attention_dkv_kernel(AttentionArgs a) {
     }
   };
   int buffer = 0;
+  const int begin = step;
   load(step, 0);
   store(0);
   while (step < stop) {
@@ -707,7 +729,7 @@ attention_dkv_kernel(AttentionArgs a) {
     int until = min(stop, step - step % tiles + tiles - masked);
     for (; step < until; ++step, buffer ^= 1) {
       arrived();
-      tile.template operator()<false>(step, buffer);
+      tile.template operator()<false, false>(step, step + 1, buffer);
       store(buffer ^ 1);
     }
     if (!CAUSAL) continue;
@@ -719,7 +741,25 @@ attention_dkv_kernel(AttentionArgs a) {
       if (first + kLines - 1 < wave_key)
         load(step + 1, buffer ^ 1);
       else
-        tile.template operator()<true>(step, buffer);
+        tile.template operator()<true, false>(step, step + 1, buffer);
+      store(buffer ^ 1);
+    }
+  }
+  // the last tiles of each head, whose rows see few keys
+  const int few = n <= kFewKeys ? tiles
+                  : CAUSAL      ? min(tiles, max(0, kFewKeys - start) / kLines)
+                                : 0;
+  if (!SHORT && few && begin < stop) {
+    auto from = [&](int step) {  // the first of these that is not before `step`
+      return step + max(0, tiles - few - step % tiles);
+    };
+    step = from(begin);
+    __syncthreads();  // the tiles are not read any more
+    load(step, buffer);
+    store(buffer);
+    for (; step < stop; step = from(step + 1), buffer ^= 1) {
+      arrived();
+      tile.template operator()<CAUSAL, true>(step, from(step + 1), buffer);
       store(buffer ^ 1);
     }
   }
@@ -792,10 +832,10 @@ int forward(const AttentionArgs& a) {
   return a.causal ? forward<DP, true, false>(a) : forward<DP, false, false>(a);
 }
 
-template <int DP, bool CAUSAL, bool SHORT>
+template <int DP, bool CAUSAL, bool EXACT>
 int dq(const AttentionArgs& a) {
   const int64_t blocks = (a.tokens + kRows - 1) / kRows;
-  hipLaunchKernelGGL((attention_dq_kernel<DP, CAUSAL, SHORT>),
+  hipLaunchKernelGGL((attention_dq_kernel<DP, CAUSAL, EXACT>),
                      dim3((unsigned) (blocks * a.batch * a.heads)),
                      dim3(kThreads), 0, static_cast<hipStream_t>(a.stream), a);
   return (int) hipGetLastError();
@@ -813,14 +853,13 @@ int dkv(const AttentionArgs& a) {
 
 template <int DP, bool CAUSAL>
 int backward(const AttentionArgs& a) {
-  const bool is_short = a.tokens <= kShort;
-  // dQ of short heads as well, where it was 1.5 times as far off as its own
-  // rounding leaves it (1.44 from 64 elements on): 78 us in place of 62 at 2 x
-  // 2048 tokens, 32 heads of 16
-  int status = is_short || a.dim <= 32 ? dq<DP, CAUSAL, true>(a)
+  // dQ of short heads with 16 bits everywhere, where it was 1.5 times as far off as
+  // its own rounding leaves it (1.44 from 64 elements on): 78 us in place of 62 at
+  // 2 x 2048 tokens, 32 heads of 16
+  int status = DP <= 64 && a.dim <= 32 ? dq<DP, CAUSAL, DP <= 64>(a)
                                        : dq<DP, CAUSAL, false>(a);
   if (status) return status;
-  status = is_short ? dkv<DP, CAUSAL, true>(a) : dkv<DP, CAUSAL, false>(a);
+  status = a.tokens <= kFewKeys ? dkv<DP, CAUSAL, true>(a) : dkv<DP, CAUSAL, false>(a);
   if (status || a.key_parts == 1) return status;
   const int64_t threads =
       (int64_t) a.batch * a.kv_heads * a.tokens * (a.dim / 8) * 2;

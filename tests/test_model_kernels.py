@@ -423,6 +423,32 @@ def test_attention_normalizes_by_what_is_not_rounded(d):
     assert (dv[:, :, 6:] == 0.5).all()
 
 
+def roundings(got, want):
+    """How far results are off, as a multiple of what rounding the exact ones to bf16 leaves (norms)."""
+    return ((got.detach().double() - want).norm() / (want.to(BF16).double() - want).norm()).item()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("causal", [True, False])
+@pytest.mark.parametrize("d", [24, 64, 128])
+@pytest.mark.parametrize("t", [257, 700])
+def test_attention_few_keys_in_a_long_batch(t, d, causal):
+    """Gradients of rows that see up to 256 keys take 16 bits of P and dS however far their batch is padded."""
+    lengths = [200, 33, t, 256]
+    q, k, v, do = attention_case(len(lengths), 4, 2, t, d, seed=t + d)
+    valid = torch.tensor(lengths, dtype=torch.int32, device="cuda")
+    got = torch.autograd.grad(kernels.attention(q, k, v, lengths=valid, causal=causal), (q, k, v), do)
+    value, _ = attention_64(q, k, v, do, lengths, causal, 1 / math.sqrt(d))
+    # With 8 bits a second rounding of the same size joins the results' own: sqrt(2). With 16, what is left is that of
+    # the probabilities in O, by way of delta, which is less than half as large: sqrt(1 + 1 / 4) at most.
+    for name, x in zip(("dq", "dk", "dv"), got):
+        for i, n in enumerate(lengths):
+            if n <= 256:
+                assert roundings(x[i, :, :n], value[name][i, :, :n]) <= 1.2, (name, n)
+    if causal:
+        assert roundings(got[0][2, :, :256], value["dq"][2, :, :256]) <= 1.2
+
+
 @pytest.mark.gpu
 def test_attention_large_scores():
     """Scores in the hundreds: a softmax that is almost a choice; a scale of the caller's."""
