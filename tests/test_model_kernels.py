@@ -428,6 +428,57 @@ def roundings(got, want):
     return ((got.detach().double() - want).norm() / (want.to(BF16).double() - want).norm()).item()
 
 
+def farthest_head(got, want):
+    """|got - want| / |want| as norms over the tokens of a head, the largest of them."""
+    return ((got.detach().double() - want).norm(dim=(-2, -1)) / want.norm(dim=(-2, -1))).max().item()
+
+
+# Where the bounds of values add up a whole row's roundings, norms tell more. Roundings of independent sign, each evenly
+# spread over u of its value (u / sqrt(3)): the result's own, that of P or dS, and that of the probabilities in O, which
+# reaches the gradients by way of delta: sqrt(3) u / sqrt(3).
+LONG_ROWS = U[BF16]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("causal", [True, False])
+@pytest.mark.parametrize("h, kv, t, d", [(2, 1, 2000, 128), (4, 2, 1025, 64), (2, 2, 513, 40), (3, 1, 4096, 64), (2, 1, 700, 16)])
+def test_attention_long_rows(h, kv, t, d, causal):
+    q, k, v, do = attention_case(1, h, kv, t, d, seed=t + 1)
+    o = kernels.attention(q, k, v, causal=causal)
+    grads = torch.autograd.grad(o, (q, k, v), do)
+    value, _ = attention_64(q, k, v, do, None, causal, 1 / math.sqrt(d))
+    for name, x in zip(("o", "dq", "dk", "dv"), (o, *grads)):
+        assert farthest_head(x, value[name]) <= LONG_ROWS, name
+
+
+@pytest.mark.parametrize("causal", [True, False])
+def test_norms_of_long_rows_tell_mistakes(causal):
+    """Planted in the formulas, on the CPU: each is beyond what test_attention_long_rows allows."""
+    g = torch.Generator().manual_seed(3)
+    t, d = 600, 64
+    q, k, v, do = (torch.randn(t, d, generator=g).to(BF16).double() for _ in range(4))
+
+    def gradients(of_delta=1.0, lse=0.0, keys=t, rows=t):
+        s = q @ k.t() / math.sqrt(d)
+        if causal:
+            s = s.masked_fill(torch.ones(t, t, dtype=torch.bool).triu(1), -math.inf)
+        exact = torch.softmax(s, -1)
+        p, delta = exact * math.exp(lse), (do * (exact @ v)).sum(-1, keepdim=True)
+        ds = p * (do @ v.t() - of_delta * delta) / math.sqrt(d)
+        return {"dq": ds[:, :keys] @ k[:keys], "dk": ds[:rows].t() @ q[:rows], "dv": p[:rows].t() @ do[:rows]}
+
+    want = gradients()
+    for mistake, wrong in (
+        (dict(of_delta=0.0), ("dq", "dk")), (dict(of_delta=0.9), ("dq", "dk")), (dict(lse=0.01), ("dq", "dk", "dv")),
+        (dict(keys=t - 32), ("dq",)), (dict(rows=t - 32), ("dk", "dv")),
+    ):
+        got = gradients(**mistake)
+        for name in wrong:
+            assert farthest_head(got[name], want[name]) > LONG_ROWS, (mistake, name)
+    for name, x in want.items():
+        assert farthest_head(x * 1.01, x) > LONG_ROWS and farthest_head(x.to(BF16), x) < LONG_ROWS
+
+
 @pytest.mark.gpu
 @pytest.mark.parametrize("causal", [True, False])
 @pytest.mark.parametrize("d", [24, 64, 128])
