@@ -33,15 +33,55 @@ def _newer(dst: str, *srcs: str) -> bool:
     return all(os.path.getmtime(s) <= dt for s in srcs if os.path.exists(s))
 
 
-def _run(cmd, verbose=False):
+def _recipe(cmd, *uses: str) -> str:
+    """What a target depends on besides its sources, wherever the tree is: the
+    command, the ROCm release, and `uses`."""
+    try:
+        with open(os.path.join(ROCM, ".info", "version")) as f:
+            rocm = f.read().strip()
+    except OSError:
+        rocm = "unknown"
+    return "\n".join([*cmd, *uses, "ROCm " + rocm]).replace(HERE, ".") + "\n"
+
+
+def _fresh(dst: str, srcs, recipe: str) -> bool:
+    """dst is newer than srcs and was made by the same recipe, which is kept
+    beside it."""
+    try:
+        with open(dst + ".made") as f:
+            return f.read() == recipe and _newer(dst, *srcs)
+    except OSError:
+        return False
+
+
+def _start(cmd, verbose: bool) -> subprocess.Popen:
     if verbose:
         print("+ " + " ".join(cmd))
-    subprocess.run(cmd, check=True)
+    return subprocess.Popen(cmd)
 
 
-def build_all(verbose: bool = False, model: bool = True) -> None:
+def _finish(running) -> None:
+    """Waits for all (dst, recipe, cmd, process), then raises if one failed."""
+    failed = None
+    for dst, recipe, cmd, process in running:
+        if process.wait() != 0:
+            failed = failed or (process.returncode, cmd)
+        else:
+            with open(dst + ".made", "w") as f:
+                f.write(recipe)
+    if failed:
+        raise subprocess.CalledProcessError(*failed)
+
+
+def _make(dst: str, srcs, cmd, verbose: bool, force: bool, *uses: str) -> None:
+    recipe = _recipe(cmd, *uses)
+    if force or not _fresh(dst, srcs, recipe):
+        _finish([(dst, recipe, cmd, _start(cmd, verbose))])
+
+
+def build_all(verbose: bool = False, model: bool = True, force: bool = False) -> None:
     """model: the operators of workloads.kernels as well, which recording does
-    not need and which take a minute."""
+    not need and which take a minute.  force: also what is up to date."""
     os.makedirs(BIN, exist_ok=True)
     os.makedirs(LIB, exist_ok=True)
 
@@ -121,10 +161,8 @@ def build_all(verbose: bool = False, model: bool = True) -> None:
     for dst, srcs, cc, link in host_targets:
         if not os.path.exists(srcs[0]):
             continue
-        if _newer(dst, *srcs):
-            continue
         cc_srcs = [s for s in srcs if s.endswith((".cc", ".cpp"))]
-        _run(cc + ["-o", dst] + cc_srcs + link, verbose)
+        _make(dst, srcs, cc + ["-o", dst] + cc_srcs + link, verbose, force)
 
     # --- HIP device code (gfx950) ---
     hipcc = os.path.join(ROCM, "bin", "hipcc")
@@ -148,8 +186,6 @@ def build_all(verbose: bool = False, model: bool = True) -> None:
         srcs = [s for s in srcs if os.path.exists(s)]
         if not srcs:
             continue
-        if _newer(dst, *srcs):
-            continue
         cmd = [hipcc] + HIP_FLAGS + ["-std=c++17"]
         if dst.endswith(".so"):
             cmd += ["-fPIC", "-shared"]
@@ -157,13 +193,13 @@ def build_all(verbose: bool = False, model: bool = True) -> None:
         if dst.endswith("sofa-bandwidth"):
             # --ring mode links the device-trace-ring machinery
             cmd += ["-L" + LIB, "-lsofahip", "-Wl,-rpath,$ORIGIN/../lib"]
-        _run(cmd, verbose)
+        _make(dst, srcs, cmd, verbose, force)
 
     if model:
-        _build_model_kernels(hipcc, verbose)
+        _build_model_kernels(hipcc, verbose, force)
 
 
-def _build_model_kernels(hipcc: str, verbose: bool) -> None:
+def _build_model_kernels(hipcc: str, verbose: bool, force: bool) -> None:
     """The operators of workloads.kernels: the kernels, one object per source,
     compiled side by side (their many variants take a minute each) and linked
     into libsofamodel, and their binding to torch where torch is installed."""
@@ -173,42 +209,42 @@ def _build_model_kernels(hipcc: str, verbose: bool) -> None:
     srcs = [os.path.join(src_dir, n) for n in sorted(os.listdir(src_dir)) if n.endswith(".hip")]
     objs, running = [], []
 
-    def start(cmd):
-        if verbose:
-            print("+ " + " ".join(cmd))
-        running.append((cmd, subprocess.Popen(cmd)))
+    def start(obj, srcs, cmd, *uses):
+        recipe = _recipe(cmd, *uses)
+        if force or not _fresh(obj, srcs, recipe):
+            running.append((obj, recipe, cmd, _start(cmd, verbose)))
 
     for src in srcs:
         obj = os.path.join(LIB, os.path.basename(src)[:-4] + ".o")
         objs.append(obj)
-        if not _newer(obj, src, *headers):
-            start([hipcc] + HIP_FLAGS + ["-std=c++20", "-fPIC", "-c", src, "-o", obj])
+        start(obj, [src, *headers], [hipcc] + HIP_FLAGS + ["-std=c++20", "-fPIC", "-c", src, "-o", obj])
 
     binding = os.path.join(src_dir, "bindings.cc")
     module, module_obj = os.path.join(LIB, "sofa_model.so"), os.path.join(LIB, "bindings.o")
-    torch_lib = None
+    torch_lib = torch_version = None
     try:
         import torch
         from torch.utils.cpp_extension import include_paths
 
         torch_lib = os.path.join(os.path.dirname(torch.__file__), "lib")
+        torch_version = "torch " + torch.__version__
     except ImportError:
         if verbose:
             print("torch is not installed: the operators of workloads.kernels are not bound")
-    if torch_lib and not _newer(module_obj, binding, headers[1]):
+    if torch_lib:
         include = include_paths() + [f"{ROCM}/include", sysconfig.get_paths()["include"]]
-        start(["g++", "-O2", "-std=c++17", "-fPIC", "-fvisibility=hidden", "-D__HIP_PLATFORM_AMD__", "-DUSE_ROCM",
+        start(module_obj, [binding, headers[1]],
+              ["g++", "-O2", "-std=c++17", "-fPIC", "-fvisibility=hidden", "-D__HIP_PLATFORM_AMD__", "-DUSE_ROCM",
                f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}"]
-              + [f"-I{i}" for i in include] + ["-c", binding, "-o", module_obj])
+              + [f"-I{i}" for i in include] + ["-c", binding, "-o", module_obj], torch_version)
 
-    failed = [cmd for cmd, p in running if p.wait() != 0]
-    if failed:
-        raise subprocess.CalledProcessError(1, failed[0])
-    if not _newer(dst, *objs):
-        _run([hipcc, f"--offload-arch={GFX_ARCH}", "-shared", "-o", dst] + objs, verbose)
-    if torch_lib and not _newer(module, module_obj, dst):
-        _run(["g++", "-shared", "-o", module, module_obj, f"-L{torch_lib}", "-ltorch_python", "-ltorch", "-ltorch_cpu",
-              "-lc10_hip", "-lc10", f"-L{LIB}", "-lsofamodel", "-Wl,-rpath,$ORIGIN"], verbose)
+    _finish(running)
+    _make(dst, objs, [hipcc, f"--offload-arch={GFX_ARCH}", "-shared", "-o", dst] + objs, verbose, force)
+    if torch_lib:
+        _make(module, [module_obj, dst],
+              ["g++", "-shared", "-o", module, module_obj, f"-L{torch_lib}", "-ltorch_python", "-ltorch",
+               "-ltorch_cpu", "-lc10_hip", "-lc10", f"-L{LIB}", "-lsofamodel", "-Wl,-rpath,$ORIGIN"],
+              verbose, force, torch_version)
 
 
 if __name__ == "__main__":

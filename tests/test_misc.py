@@ -1,6 +1,7 @@
 """Small coverage tests: CPU-degradation paths of GPU-facing helpers."""
 
 import os
+import subprocess
 
 import pytest
 
@@ -61,3 +62,34 @@ def test_hsalite_library_loads():
     assert lib.sofa_lite_active() == 0
     lib.sofa_lite_event_count.restype = ctypes.c_ulonglong
     assert lib.sofa_lite_event_count() == 0
+
+
+def test_native_targets_are_made_again_when_their_recipe_changes(tmp_path, monkeypatch, capfd):
+    """Newer than its sources is not enough: flags, and what a target is linked against, count too."""
+    import time
+
+    from sofa_amd.native import build
+
+    src, dst = tmp_path / "x.cc", str(tmp_path / "x.o")
+    src.write_text("int x() { return VALUE; }\n")
+
+    def make(*flags, uses=(), force=False):
+        capfd.readouterr()
+        build._make(dst, [str(src)], ["g++", "-DVALUE=1", *flags, "-c", str(src), "-o", dst], True, force, *uses)
+        return "+ g++" in capfd.readouterr().out
+
+    assert make()
+    assert not make()
+    assert make("-O1") and not make("-O1")
+    assert make("-O1", uses=["torch 1"]) and not make("-O1", uses=["torch 1"]) and make("-O1", uses=["torch 2"])
+    assert make("-O1", uses=["torch 2"], force=True) and not make("-O1", uses=["torch 2"])
+    os.utime(src, (time.time() + 60,) * 2)
+    assert make("-O1", uses=["torch 2"])
+    os.utime(src, (time.time() - 60,) * 2)
+    # a command that fails leaves the target to be made, and another place of the tree does not
+    with pytest.raises(subprocess.CalledProcessError):
+        make("-DVALUE=(")
+    monkeypatch.setattr(build, "HERE", str(tmp_path))
+    recipe = build._recipe(["g++", f"-I{tmp_path}/include"])
+    monkeypatch.setattr(build, "HERE", "/elsewhere")
+    assert recipe == build._recipe(["g++", "-I/elsewhere/include"])
