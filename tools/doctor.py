@@ -33,7 +33,7 @@ def main():
     for b in ("sofa-cpusampler", "sofa-timebase", "sofa-pktcap", "sofa-syscalltrace"):
         check(f"native {b}", os.path.exists(os.path.join(REPO, "sofa_amd", "native", "bin", b)),
               "python -m sofa_amd.native.build")
-    for lib in ("libsofatracer.so", "libsofahip.so", "libsofamodel.so"):
+    for lib in ("libsofatracer.so", "libsofahip.so", "libsofamodel.so", "sofa_model.so"):
         check(f"native {lib}", os.path.exists(os.path.join(REPO, "sofa_amd", "native", "lib", lib)),
               "python -m sofa_amd.native.build")
     try:
