@@ -34,12 +34,15 @@
 // Measured at 32 query and 8 key heads of 128, causal, in products' TFLOP/s
 // (2, 3 and 4 products; a large library product reaches 1220):
 //                  2 x 2048      2 x 4096       1 x 8192 tokens
-//   forward        93 us  740    315 us  870    565 us  970
-//   dQ            125 us  825    440 us  935    765 us 1080
-//   dK, dV        150 us  915    580 us  950   1075 us 1020
-// What bounds them is the issue of a wave's own instructions: products take 40 %
-// of its cycles, exponentials and their surroundings as many, and two waves on
-// a SIMD (256 registers each) fill each other's gaps only in part.
+//   forward, lse  100 us  690    312 us  880    568 us  970
+//   dQ            124 us  830    416 us  990    740 us 1115
+//   dK, dV        172 us  800    555 us  990   1035 us 1065
+// What bounds them there is the issue of a wave's own instructions: products take
+// 40 % of its cycles, exponentials and their surroundings as many, and two waves
+// on a SIMD (256 registers each) fill each other's gaps only in part.  Where all
+// workgroups are resident at once (up to about 2 x 2048 of these) it is the longest
+// chain of tiles that one of them goes through.  Heads are padded to 64 or 128
+// elements, and the padding is multiplied.
 
 #include "model_ops.h"
 
@@ -288,8 +291,9 @@ __device__ __forceinline__ int valid_tokens(const AttentionArgs& a, int batch) {
 }
 
 // Short heads of long rows: four workgroups on a compute unit, at the cost of a
-// register spilled (2 x 4096 tokens, 32/8 heads of 64, no mask: 325 us in place of
-// 340 with three); a few hundred tokens do not fill them, and lose 3 %.
+// register or three spilled (2 x 4096 tokens, 32/8 heads of 64, no mask: 337 us in
+// place of 348 with three, 321 in place of 325 without lse); a few hundred tokens
+// do not fill them, and lose 3 %.
 // KEEP: with lse, whose own sum of the probabilities takes 4 % of the time.
 template <int DP, bool CAUSAL, bool SHORT, bool KEEP>
 __global__ __launch_bounds__(kThreads, DP > 64 ? 2 : SHORT ? 3 : 4)
@@ -574,7 +578,7 @@ void attention_dq_kernel(
 // such rows are gone over once more for the products of the rest: in the loop
 // over all tiles a second body, or a branch, takes 9 to 30 % (registers).  Those of
 // longer rows have one rounding each for heads of up to 32 too, where dQ has 16
-// bits: it would take 121 us in place of 80 at 2 x 2048 tokens, 32 heads of 16.
+// bits: it would take 129 us in place of 86 at 2 x 2048 tokens, 32 heads of 16.
 template <int DP, bool CAUSAL, bool SHORT>
 __global__ __launch_bounds__(kThreads, 2) void
 attention_dkv_kernel(AttentionArgs a) {
@@ -854,7 +858,7 @@ int dkv(const AttentionArgs& a) {
 template <int DP, bool CAUSAL>
 int backward(const AttentionArgs& a) {
   // dQ of short heads with 16 bits everywhere, where it was 1.5 times as far off as
-  // its own rounding leaves it (1.44 from 64 elements on): 78 us in place of 62 at
+  // its own rounding leaves it (1.44 from 64 elements on): 79 us in place of 64 at
   // 2 x 2048 tokens, 32 heads of 16
   int status = DP <= 64 && a.dim <= 32 ? dq<DP, CAUSAL, DP <= 64>(a)
                                        : dq<DP, CAUSAL, false>(a);

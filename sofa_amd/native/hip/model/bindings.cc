@@ -215,9 +215,9 @@ AttentionArgs attention_args(const Tensor& q, const Tensor& k, const Tensor& v,
 
 // Workgroups that share the rows behind one block of 128 keys. Two fit a compute
 // unit, so 512 fill the card; under a causal mask the blocks differ in work and
-// twice as many even it out (8192 tokens, 8 key heads of 128: 1.15 ms with two
-// parts, 1.71 with one). Parts cost a pass over their sums, and one of less than
-// four steps gains nothing.
+// twice as many even it out (8 key heads of 128: 8192 tokens 1040 us with two parts
+// and 25 to join them, 1810 with one; 2 x 2048 tokens 172 and 23 with four, 462 with
+// one). One of less than four steps gains nothing.
 int key_parts(int64_t batch, int64_t heads, int64_t kv_heads, int64_t tokens,
               int64_t dim, bool causal) {
   const int64_t groups = batch * kv_heads * ceil_div(tokens, 128);

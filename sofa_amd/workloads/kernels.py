@@ -8,11 +8,13 @@ All three are differentiable (first derivatives, backward mode), run on the curr
 their tensors' device, allocate what they return and nothing that outlives the
 call, give the same bits for the same inputs, and can be captured into a graph
 (a backward pass, as always with torch, while no eager graph of its leaves lives).
-They need tensors on a GPU: there is no other path, and a missing library is an
+They are operators of torch's dispatcher (torch.ops.sofa_model), which its tracers
+record.  They need tensors on a GPU: there is no other path, and a missing library is an
 error.  Wrong arguments raise TypeError (types) or ValueError (shapes, values).
 
 `Llama(kernels="hip")` and `python -m sofa_amd.workloads.llama --kernels hip`
-run the decoder on them.  The kernels are in native/hip/model.
+run the decoder on them, under bfloat16 autocast or with bfloat16 weights.  The
+kernels are in native/hip/model.
 """
 
 from __future__ import annotations
@@ -77,8 +79,8 @@ def attention(
     q is (batch, heads, tokens, dim); k and v are (batch, kv_heads, tokens, dim),
     where kv_heads divides heads and query head i reads key head
     i // (heads // kv_heads).  All are bfloat16; dim is a multiple of 8 up to
-    128; any strides (rows that are not dense or not at multiples of 16 bytes
-    are copied first).  scale is above 0 (1e-18 to 1e18), 1 / sqrt(dim) if not given.
+    128, and computed as if it were 64 or 128; any strides (rows that are not dense
+    or not at multiples of 16 bytes are copied first).  scale is above 0 (1e-18 to 1e18), 1 / sqrt(dim) if not given.
 
     causal: token i sees tokens 0..i, otherwise all.  lengths: int32 (batch,),
     the valid tokens at the front of each sequence, taken as within 0..tokens;
@@ -89,6 +91,11 @@ def attention(
     float16 is refused: the gradient of a score, which the products of the
     backward pass take in the inputs' type, is below float16's smallest normal
     value in long sequences.
+
+    Scores are sums of 32 bits: one of size s is off by some 2^-24 s, and its
+    probability by that share.  The products of probabilities, and in rows that see
+    more than 256 keys those of the scores' gradients, take them rounded to bfloat16;
+    a score's gradient is good to 2^-17 of the gradient of its probability.
 
     Returns (batch, heads, tokens, dim), laid out as (batch, tokens, heads, dim).
     For a backward pass q, k, v and twice the size of the result are kept.
