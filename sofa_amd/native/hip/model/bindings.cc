@@ -301,6 +301,7 @@ struct Attention : torch::autograd::Function<Attention> {
                         const Tensor& k_in, const Tensor& v_in,
                         const Optional& lengths, double scale, bool causal) {
     const Below below;
+    check_attention(q_in, k_in, v_in, unpack(lengths));  // before strides are read
     const Tensor q = rows16(q_in), k = rows16(k_in), v = rows16(v_in);
     const auto [o, o_low, lse] =
         op<&attention_forward>("sofa_model::attention_forward")

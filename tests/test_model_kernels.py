@@ -204,6 +204,21 @@ def test_dispatched_operators_check_what_they_are_given(ops):
             torch.ops.sofa_model.residual_norm_backward(*args)
 
 
+@pytest.mark.parametrize("name", ["attention", "token_logprobs", "token_logprobs_top", "residual_norm", "rms_norm"])
+def test_dispatched_operators_check_before_they_record(ops, name):
+    """The same where a backward pass is recorded, and inputs are laid out for it first."""
+    f, args = getattr(torch.ops.sofa_model, name), _meta_step()[name]
+    args = [t.requires_grad_() if isinstance(t, torch.Tensor) and t.is_floating_point() else t for t in args]
+    out = f(*args)
+    assert (out if isinstance(out, torch.Tensor) else out[0]).requires_grad
+    for i, t in enumerate(args):
+        if not isinstance(t, torch.Tensor) or (name == "rms_norm" and i == 0):
+            continue
+        for wrong in (t[0], t[1:], t[None], t.flatten()[0], t.to(torch.float64)):
+            with pytest.raises((RuntimeError, IndexError), match="does not belong|the model kernels have no|Dimension"):
+                f(*args[:i], wrong, *args[i + 1:])
+
+
 def test_fake_tensors_and_make_fx(ops):
     """Shapes, types and layouts without data, and each operator as a node of a recorded graph."""
     from torch._subclasses.fake_tensor import FakeTensorMode
